@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define PLC_VERSION 102
+#define PLC_VERSION 103
 
 enum {
     PLC_OK = 0,
@@ -391,6 +391,111 @@ int plc_dp_pack_grads(const plc_opt_tensor* t, int n, float* flat, long long fla
                       const float* guard, void* stream);
 int plc_dp_unpack_grads(const plc_opt_tensor* t, int n, const float* flat, long long flat_elems,
                         const float* guard_in, float* guard_out, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Layer operators.  No counterpart in the reference: what a recurrent conv model is commonly extended with around
+ * its ConvLSTM cells -- a recurrence whose gates do not depend on the state (so that long sequences need no step by
+ * step evaluation), group norm with an activation, dropout.
+ *
+ * Element types of x, f, y and of the gradients of these: PLC_F32, PLC_BF16, PLC_F16; everything that is summed or
+ * carried (states, statistics, gradients of norm weights) is fp32.  Tensors need the alignment of their elements only
+ * (16-byte aligned ones with strides that are multiples of 16 bytes take the wide accesses).  Empty sizes are
+ * allowed and launch nothing, except that norm weight gradients over nothing are set to 0.
+ * ------------------------------------------------------------------------------------- */
+enum { PLC_F32 = 0, PLC_BF16 = 1, PLC_F16 = 2 };
+
+/* Gated linear recurrence over t = 0 .. T - 1, elementwise in (b, d):
+ *   s_t = sigmoid(f_t);  coupled: h_t = s_t h_{t-1} + (1 - s_t) x_t;  else h_t = s_t h_{t-1} + x_t;  y_t = h_t
+ * x, f (and dy) are [B][T][D] with D contiguous and the given element strides of a sample and of a step (0 repeats
+ * one); y, dx, df are contiguous [B][T][D]; h0, h_last, dh_last, dh0 are fp32 [B][D].
+ *   lengths  NULL or int32 [B] on the device: sample b has min(max(lengths[b], 0), T) steps.  Behind them y, dx and df
+ *            are 0, whatever x, f and dy hold there, and the state stands still (h_last of a sample without a step is h0).
+ *   h0       NULL = zeros;  h_last NULL = not wanted, else it may be h0 itself (a state updated in place)
+ *   states   forward: NULL, or room for plc_gated_scan_states_bytes(B, T, D) bytes that the backward pass reads
+ *            (the fp32 state in front of every 16th step; none for T <= 16, where NULL serves the backward pass too)
+ * Backward (dh_last, dh0 may be NULL): g_t = dy_t + s_{t+1} g_{t+1}, g behind the last step = dh_last;
+ *   coupled: dx_t = (1 - s_t) g_t, df_t = g_t (h_{t-1} - x_t) s_t (1 - s_t);  else dx_t = g_t, df_t = g_t h_{t-1} s_t (1 - s_t);
+ *   dh0 = s_0 g_0.  The states are rebuilt in fp32 from x, f and `states`; y is not read.
+ * Results do not depend on anything but the inputs and sizes (no atomics).  T = 1 is the single-step form. */
+typedef struct plc_scan_desc {
+    int B, T;
+    long long D;
+    int dtype;
+    int coupled;
+    const void* x; long long x_batch, x_step;
+    const void* f; long long f_batch, f_step;
+    const float* h0;
+    const int* lengths;
+    void* y;
+    float* h_last;
+    float* states;
+    /* backward only */
+    const void* dy; long long dy_batch, dy_step;
+    const float* dh_last;
+    void* dx;
+    void* df;
+    float* dh0;
+    /* plc_gated_scan_workspace_bytes(desc, backward) bytes, 16-byte aligned (NULL when that is 0) */
+    void* workspace;
+    size_t workspace_bytes;
+} plc_scan_desc;
+
+size_t plc_gated_scan_states_bytes(int B, int T, long long D);
+size_t plc_gated_scan_workspace_bytes(const plc_scan_desc* d, int backward);
+int plc_gated_scan_fwd(const plc_scan_desc* d, void* stream);
+int plc_gated_scan_bwd(const plc_scan_desc* d, void* stream);
+
+/* Dropout from a counter-based generator (Philox4x32-10); the mask is a function of (seed, offset, element) and is
+ * never stored, so the backward pass is the same call on dy.
+ *   thr = floor(65536 p + 0.5);  element e stays when the 16-bit value e & 7 (low half of word 0 first) of
+ *   Philox(counter words = (e >> 3 low, high, offset low, high), key words = (seed low, high)) is >= thr;
+ *   y = (stays ? x * 65536 / (65536 - thr) : 0) + residual          (a dropped element is 0 even where x is not finite)
+ *   residual     NULL or a tensor of x's type
+ *   offset_ptr   NULL, or a device int64 that is read when the kernel runs and takes the place of `offset`: a captured
+ *                graph whose program advances it draws a new mask on every replay
+ *   used_offset  NULL, or a device int64 that receives the offset this call used (what the backward pass is given) */
+int plc_dropout(const void* x, const void* residual, void* y, long long n, int dtype, double p,
+                unsigned long long seed, unsigned long long offset, const long long* offset_ptr, long long* used_offset,
+                void* stream);
+
+/* Group norm over the HW pixels and C / G channels of each group of each of N samples, with an activation and, when
+ * p > 0, dropout in the same pass:
+ *   xh = (x - mean) / sqrt(var + eps);  z = weight_c xh + bias_c;  y = dropout(act(z))
+ * layout: PLC_NHWC = [N][HW][C], PLC_CB8 = [N][C/8][HW][8] (the engine's activations; C a multiple of 8).  Dropout
+ * counts elements in [N][HW][C] order in both.
+ *   weight, bias  fp32 [C] or NULL (1, 0);  stats: fp32 [N][G][2] (mean, 1 / sqrt(var + eps)), written by the forward
+ *                 and read by the backward pass
+ *   dweight, dbias  fp32 [C] or NULL, overwritten
+ * The backward pass takes the same x, weight, bias, p, seed and the offset the forward pass used.  ReLU's slope at 0
+ * is 0.  Sums run in a fixed order (bit-repeatable). */
+enum { PLC_ACT_NONE = 0, PLC_ACT_RELU = 1, PLC_ACT_SILU = 2 };
+enum { PLC_NHWC = 0, PLC_CB8 = 1 };
+typedef struct plc_norm_desc {
+    int N, C, G, HW;
+    int dtype, layout, act;
+    float eps;
+    const void* x;
+    const float* weight;
+    const float* bias;
+    void* y;
+    float* stats;
+    double p;
+    unsigned long long seed, offset;
+    const long long* offset_ptr;   /* as plc_dropout */
+    long long* used_offset;
+    /* backward only */
+    const void* dy;
+    void* dx;
+    float* dweight;
+    float* dbias;
+    /* plc_group_norm_workspace_bytes(desc) bytes, 16-byte aligned */
+    void* workspace;
+    size_t workspace_bytes;
+} plc_norm_desc;
+
+size_t plc_group_norm_workspace_bytes(const plc_norm_desc* d);
+int plc_group_norm_fwd(const plc_norm_desc* d, void* stream);
+int plc_group_norm_bwd(const plc_norm_desc* d, void* stream);
 
 #ifdef __cplusplus
 }

@@ -12,7 +12,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # (PLC_LIB_PATH: load another build of the library instead, e.g. an older one for a same-box comparison)
 LIB_PATH = os.environ.get("PLC_LIB_PATH") or os.path.join(_HERE, "libplconvlstm.so")
 
-ABI_VERSION = 102      # PLC_VERSION of the include/plconvlstm.h these bindings mirror
+ABI_VERSION = 103      # PLC_VERSION of the include/plconvlstm.h these bindings mirror
 EXPORTS = (
     "plc_version", "plc_last_error",
     "plc_nchw_f32_to_cb8_bf16", "plc_cb8_bf16_to_nchw_f32", "plc_nchw_f32_to_cb8_f32", "plc_cb8_f32_to_nchw_f32",
@@ -27,6 +27,8 @@ EXPORTS = (
     "plc_combined_loss_workspace_bytes", "plc_combined_loss",
     "plc_clip_adam_workspace_bytes", "plc_clip_adam_step", "plc_clip_adam_step_guarded",
     "plc_dp_pack_grads", "plc_dp_unpack_grads",
+    "plc_gated_scan_states_bytes", "plc_gated_scan_workspace_bytes", "plc_gated_scan_fwd", "plc_gated_scan_bwd",
+    "plc_dropout", "plc_group_norm_workspace_bytes", "plc_group_norm_fwd", "plc_group_norm_bwd",
 )
 
 _f = C.c_void_p   # device pointers travel as plain addresses
@@ -89,6 +91,26 @@ class PointwiseBwdArgs(C.Structure):
     """Mirror of ``plc_pointwise_bwd_args``."""
     _fields_ = [("dh0", _f), ("dh0_image_bytes", C.c_longlong), ("dh1", _f), ("dh1_image_bytes", C.c_longlong),
                 ("dc_next", _f), ("gates", _f), ("c_prev", _f), ("dz", _f), ("dc", _f), ("Ch", C.c_int)]
+
+
+class ScanDesc(C.Structure):
+    """Mirror of ``plc_scan_desc``."""
+    _fields_ = [("B", C.c_int), ("T", C.c_int), ("D", C.c_longlong), ("dtype", C.c_int), ("coupled", C.c_int),
+                ("x", _f), ("x_batch", C.c_longlong), ("x_step", C.c_longlong),
+                ("f", _f), ("f_batch", C.c_longlong), ("f_step", C.c_longlong),
+                ("h0", _f), ("lengths", _f), ("y", _f), ("h_last", _f), ("states", _f),
+                ("dy", _f), ("dy_batch", C.c_longlong), ("dy_step", C.c_longlong),
+                ("dh_last", _f), ("dx", _f), ("df", _f), ("dh0", _f), ("workspace", _f), ("workspace_bytes", C.c_size_t)]
+
+
+class NormDesc(C.Structure):
+    """Mirror of ``plc_norm_desc``."""
+    _fields_ = [("N", C.c_int), ("C", C.c_int), ("G", C.c_int), ("HW", C.c_int),
+                ("dtype", C.c_int), ("layout", C.c_int), ("act", C.c_int), ("eps", C.c_float),
+                ("x", _f), ("weight", _f), ("bias", _f), ("y", _f), ("stats", _f),
+                ("p", C.c_double), ("seed", C.c_ulonglong), ("offset", C.c_ulonglong),
+                ("offset_ptr", _f), ("used_offset", _f),
+                ("dy", _f), ("dx", _f), ("dweight", _f), ("dbias", _f), ("workspace", _f), ("workspace_bytes", C.c_size_t)]
 
 
 _lib = None
@@ -177,6 +199,19 @@ def lib():
     L.plc_dp_pack_grads.argtypes = [C.POINTER(OptTensor), i, p, C.c_longlong, C.c_float, p, p]
     L.plc_dp_unpack_grads.restype = i
     L.plc_dp_unpack_grads.argtypes = [C.POINTER(OptTensor), i, p, C.c_longlong, p, p, p]
+    L.plc_gated_scan_states_bytes.restype = sz
+    L.plc_gated_scan_states_bytes.argtypes = [i, i, C.c_longlong]
+    L.plc_gated_scan_workspace_bytes.restype = sz
+    L.plc_gated_scan_workspace_bytes.argtypes = [C.POINTER(ScanDesc), i]
+    L.plc_dropout.restype = i
+    L.plc_dropout.argtypes = [p, p, p, C.c_longlong, i, C.c_double, C.c_ulonglong, C.c_ulonglong, p, p, p]
+    L.plc_group_norm_workspace_bytes.restype = sz
+    L.plc_group_norm_workspace_bytes.argtypes = [C.POINTER(NormDesc)]
+    for name, desc in (("plc_gated_scan_fwd", ScanDesc), ("plc_gated_scan_bwd", ScanDesc),
+                       ("plc_group_norm_fwd", NormDesc), ("plc_group_norm_bwd", NormDesc)):
+        fn = getattr(L, name)
+        fn.restype = i
+        fn.argtypes = [C.POINTER(desc), p]
     _lib = L
     return L
 

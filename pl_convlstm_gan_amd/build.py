@@ -6,7 +6,8 @@ import os
 import subprocess
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SRC = os.path.join(HERE, "csrc", "plc_api.hip")
+# (the rollout engine, then the layer operators: two translation units, compiled side by side)
+SRCS = [os.path.join(HERE, "csrc", "plc_api.hip"), os.path.join(HERE, "csrc", "plc_layers.hip")]
 OUT = os.path.join(HERE, "libplconvlstm.so")
 DEPS = sorted(glob.glob(os.path.join(HERE, "csrc", "*.h")) + glob.glob(os.path.join(HERE, "csrc", "*.hip"))) + \
        [os.path.join(os.path.dirname(HERE), "include", "plconvlstm.h"), os.path.abspath(__file__)]
@@ -23,18 +24,26 @@ def build(force: bool = False, verbose: bool = True) -> str:
     if not force and not is_stale():
         return OUT
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    # -fno-slp-vectorize: the compiler must not pair scalar fp32 arithmetic into packed instructions on its own.
-    # On the MI355X a packed fp32 instruction whose SECOND source takes its low half from the high dword
-    # (v_pk_fma_f32 ... op_sel:[0,1,0], v_pk_add_f32 ... op_sel:[0,1]) gives wrong results now and then while an
-    # MFMA kernel runs on the chip at the same time (devtools/pk_opsel_probe.hip: 1.5e-4 of the instructions;
-    # never alone; the plain, op_sel_hi-only, first- and third-source forms never), and the pairing produced
-    # such encodings.  The rollouts run several kernels at once, so the library holds no packed fp32 instruction
-    # except the hand-written plain ones of the one-channel weight gradient (tests/test_host_logic.py checks the
-    # built code object).  Measured cost of the flag: none (c3 / p2 / c1, train and forward, same box).
-    cmd = [hipcc, "-O3", "--offload-arch=gfx950", "-std=c++17", "-fno-slp-vectorize", "-shared", "-fPIC", "-o", OUT, SRC]
+    # No packed fp32 arithmetic: on the MI355X a packed fp32 instruction whose SECOND source takes its low half from the
+    # high dword (v_pk_fma_f32 ... op_sel:[0,1,0], v_pk_add_f32 ... op_sel:[0,1]) gives wrong results now and then while
+    # an MFMA kernel runs on the chip at the same time (devtools/pk_opsel_probe.hip: 1.5e-4 of the instructions; never
+    # alone), and the compiler forms such encodings from ordinary scalar code and from vector types.
+    # -fno-slp-vectorize keeps it from pairing scalar arithmetic, the target feature takes the instructions away
+    # (tests/test_host_logic.py checks the built code object).  Measured cost of both: none (default train step 21.73 ms
+    # without the instructions, 21.76 with the hand-paired ones; forward 5.11 and 5.12).
+    flags = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fno-slp-vectorize", "-fPIC",
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+    objs = [os.path.splitext(src)[0] + ".o" for src in SRCS]
+    cmds = [[hipcc, *flags, "-c", "-o", obj, src] for src, obj in zip(SRCS, objs)]
+    link = [hipcc, "--offload-arch=gfx950", "-shared", "-o", OUT, *objs]
     if verbose:
-        print(" ".join(cmd), flush=True)
-    subprocess.run(cmd, check=True)
+        for cmd in cmds + [link]:
+            print(" ".join(cmd), flush=True)
+    running = [subprocess.Popen(cmd) for cmd in cmds]
+    failed = [cmd for cmd, proc in zip(cmds, running) if proc.wait() != 0]
+    if failed:
+        raise subprocess.CalledProcessError(1, failed[0])
+    subprocess.run(link, check=True)
     return OUT
 
 

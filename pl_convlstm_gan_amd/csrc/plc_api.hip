@@ -9,7 +9,7 @@
 
 #include <mutex>
 
-#include "../../include/plconvlstm.h"
+#include "plc_host.h"
 #include "plc_conv_kernel.h"
 #include "plc_convg_kernel.h"
 #include "plc_convr_kernel.h"
@@ -22,7 +22,7 @@
 // ---------------------------------------------------------------------------------------------
 static thread_local char g_err[512] = "";
 
-static int plc_fail(int code, const char* fmt, ...) {
+int plc_fail(int code, const char* fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(g_err, sizeof(g_err), fmt, ap);
@@ -30,20 +30,6 @@ static int plc_fail(int code, const char* fmt, ...) {
     return code;
 }
 
-#define PLC_HIP(expr)                                                                         \
-    do {                                                                                      \
-        hipError_t e_ = (expr);                                                               \
-        if (e_ != hipSuccess) return plc_fail(PLC_EHIP, "%s: %s", #expr, hipGetErrorString(e_)); \
-    } while (0)
-
-#define PLC_REQUIRE(cond, ...)                              \
-    do {                                                    \
-        if (!(cond)) return plc_fail(PLC_EINVAL, __VA_ARGS__); \
-    } while (0)
-
-static inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-static inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
-static inline int cdiv(int a, int b) { return (a + b - 1) / b; }
 // Channel counts inside the engine are whole 8-channel blocks: a width that is not a multiple of 8 is carried
 // with zero channels up to the next multiple (zero weights and biases keep them zero through every layer: a
 // padding channel of a ConvLSTM cell has i = f = o = 1/2, g = 0, hence c = h = 0 for ever).
@@ -252,6 +238,7 @@ static int cu_count() {
     }
     return cached[dev];
 }
+int plc_cu_count() { return cu_count(); }
 
 // Raises a kernel's dynamic-LDS limit once per (kernel, device) instead of on every launch; `done` is
 // the per-instantiation flag array of the caller.

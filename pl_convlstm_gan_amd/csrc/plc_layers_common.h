@@ -1,0 +1,99 @@
+// Device helpers of the layer operators (gated linear recurrence, group norm, dropout): element types, vector
+// loads and stores, the sigmoid, the counter-based generator.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+typedef __bf16 plc_bf16;
+typedef _Float16 plc_f16;
+
+// V consecutive elements of T, moved as one access of V * sizeof(T) bytes (16 at most; wider ones as several)
+template <class T, int V>
+struct alignas(V * sizeof(T) > 16 ? 16 : V * sizeof(T)) PlcVec {
+    T e[V];
+};
+
+template <class T, int V>
+__device__ __forceinline__ PlcVec<T, V> plc_load(const T* p) {
+    return *reinterpret_cast<const PlcVec<T, V>*>(p);
+}
+template <class T, int V>
+__device__ __forceinline__ void plc_store(T* p, const PlcVec<T, V>& v) {
+    *reinterpret_cast<PlcVec<T, V>*>(p) = v;
+}
+// (conversions from fp32 round to nearest even: results and gradients leave in the inputs' type, rounded once)
+template <class T, int V>
+__device__ __forceinline__ void plc_to_float(const PlcVec<T, V>& v, float (&o)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = (float)v.e[i];
+}
+template <class T, int V>
+__device__ __forceinline__ PlcVec<T, V> plc_from_float(const float (&v)[V]) {
+    PlcVec<T, V> o;
+#pragma unroll
+    for (int i = 0; i < V; ++i) o.e[i] = (T)v[i];
+    return o;
+}
+
+// exp(x) for x <= 0, to about one unit in the last place: the product x log2(e) is taken in two parts, so that the
+// rounding of its leading part does not grow with |x| (v_exp_f32 alone would be off by |x| 2^-24).
+__device__ __forceinline__ float plc_exp_neg(float x) {
+    const float t = x * 1.44269504088896341f;
+    // the rest of the product; t is -inf when x is, where the difference has no value
+    const float lo = __builtin_fmaf(x, 1.44269504088896341f, -t) + x * 1.92596299112661746e-8f;
+    const float e = __builtin_amdgcn_exp2f(t);
+    return t < -126.0f ? e : __builtin_fmaf(e * 0.693147180559945309f, lo, e);
+}
+
+// s = sigmoid(x) and q = 1 - s = sigmoid(-x), each to a few units in ITS last place (q is not formed by
+// subtraction: a gate near 1 would lose it).  Infinities give 0 and 1, NaN stays NaN.
+__device__ __forceinline__ void plc_sigmoid_pair(float x, float& s, float& q) {
+    const float e = plc_exp_neg(-__builtin_fabsf(x));
+    const float r = __builtin_amdgcn_rcpf(1.0f + e);
+    const float er = e * r;
+    const bool pos = x >= 0.0f;
+    s = pos ? r : er;
+    q = pos ? er : r;
+}
+
+// Philox4x32-10 (Salmon, Moraes, Dror, Shaw: Parallel random numbers: as easy as 1, 2, 3; SC 2011): 128 random bits
+// that depend on the counter and the key alone.
+__device__ __forceinline__ uint4 plc_philox(uint64_t lo, uint64_t hi, uint64_t key) {
+    uint32_t c0 = (uint32_t)lo, c1 = (uint32_t)(lo >> 32), c2 = (uint32_t)hi, c3 = (uint32_t)(hi >> 32);
+    uint32_t k0 = (uint32_t)key, k1 = (uint32_t)(key >> 32);
+#pragma unroll
+    for (int i = 0; i < 10; ++i) {
+        const uint64_t m0 = (uint64_t)0xD2511F53u * c0, m1 = (uint64_t)0xCD9E8D57u * c2;
+        c0 = (uint32_t)(m1 >> 32) ^ c1 ^ k0;
+        c2 = (uint32_t)(m0 >> 32) ^ c3 ^ k1;
+        c1 = (uint32_t)m1;
+        c3 = (uint32_t)m0;
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
+    }
+    return make_uint4(c0, c1, c2, c3);
+}
+
+// What decides which elements are dropped: element e of the tensor takes the 16-bit value e & 7 of
+// Philox(counter = (e >> 3, offset), key = seed) and stays when that is at least `thr`.  16 bits resolve a
+// probability to 2^-17; the scale is formed from the resolved one, so the mean is kept exactly.  One call of the
+// generator (about 20 quarter-rate multiplies) then serves eight elements: with 32 bits per element the
+// generator and not the memory would bound a 16-bit tensor.
+struct PlcDrop {
+    uint64_t seed, offset;
+    uint32_t thr;         // 0: nothing is dropped, 65536: everything
+    float scale;          // 65536 / (65536 - thr)
+};
+// bit i: element e0 + i stays (i < V; e0 is a multiple of V, so its V values lie in one call)
+template <int V>
+__device__ __forceinline__ uint32_t plc_keep_bits(const PlcDrop& d, uint64_t e0) {
+    const uint4 r = plc_philox(e0 >> 3, d.offset, d.seed);
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t u = (i & 1) ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu;
+        bits |= (u >= d.thr ? 1u : 0u) << i;
+    }
+    return bits >> (uint32_t)(e0 & 7);
+}

@@ -1,0 +1,163 @@
+"""Layer operators beside the ConvLSTM cell: a gated linear recurrence over long sequences, group norm with an
+activation on channels-last tensors, and dropout whose mask is computed from a counter instead of being stored.
+
+None has a counterpart in the reference.  All are HIP kernels of libplconvlstm (include/plconvlstm.h, "Layer
+operators"); float32, bfloat16 and float16 tensors, states, statistics and sums in float32.  They are differentiable
+once, run on the current stream of their tensors' device, and can be captured into a HIP graph.
+"""
+from __future__ import annotations
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import ops
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+
+
+# ------------------------------------------------------------------------------------ gated linear recurrence
+class _ScanFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, f, h0, lengths, coupled):
+        y, h_last, states = ops.gated_scan_forward(x, f, h0, lengths, coupled, save_states=True)
+        ctx.save_for_backward(x, f, h0, lengths, states)
+        ctx.coupled = coupled
+        ctx.set_materialize_grads(False)
+        return y, h_last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh_last):
+        x, f, h0, lengths, states = ctx.saved_tensors
+        if dy is None and dh_last is None:
+            return (None,) * 5
+        dx, df, dh0 = ops.gated_scan_backward(x, f, h0, lengths, ctx.coupled, states, dy, dh_last, ctx.needs_input_grad[2])
+        return dx, df, dh0, None, None
+
+
+def gated_linear_scan(x, f, h0=None, lengths=None, coupled=True):
+    """h_t = s_t h_{t-1} + (1 - s_t) x_t (``coupled``) or h_t = s_t h_{t-1} + x_t, s = sigmoid(f), elementwise over
+    [B, T, ...]; returns (h of every step in x's type, last state in float32 [B, ...]).
+
+    ``h0``: float32 [B, ...], the state in front of the first step (default zeros).  ``lengths``: int32 [B] on x's
+    device; behind a sample's length the outputs and gradients are 0, whatever the padding holds, and its state stands
+    still.  Strided x and f are read in place as long as their trailing dimensions are contiguous."""
+    if _wants_grad(x, f, h0):
+        return _ScanFn.apply(x, f, h0, lengths, bool(coupled))
+    return ops.gated_scan_forward(x, f, h0, lengths, coupled)[:2]
+
+
+def gated_linear_step(x, f, state, coupled=True, inplace=False):
+    """One step of gated_linear_scan for serving, without gradients: x, f [B, ...], ``state`` float32 [B, ...];
+    returns (h in x's type, new state).  ``inplace``: the new state overwrites ``state``."""
+    x, f = (ops._require_layer(t, n).detach() for t, n in ((x, "x"), (f, "f")))
+    state = ops._require_layer(state, "state", x, torch.float32).detach()
+    if inplace and not state.is_contiguous():
+        raise ValueError("a state that is updated in place must be contiguous")
+    y, new, _ = ops.gated_scan_forward(x.unsqueeze(1), f.unsqueeze(1), state, None, coupled, h_last=state if inplace else None)
+    return y.squeeze(1), new
+
+
+# ------------------------------------------------------------------------------------ dropout
+def _used_offset(offset):
+    return torch.empty_like(offset) if isinstance(offset, torch.Tensor) else None
+
+
+class _DropoutFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, seed, offset):
+        used = _used_offset(offset)
+        y = ops.dropout_forward(x, p, seed, offset, residual, used)
+        ctx.args = (p, seed, None if used is not None else offset)
+        ctx.save_for_backward(used)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        (used,) = ctx.saved_tensors
+        p, seed, offset = ctx.args
+        dx = ops.dropout_forward(dy, p, seed, used if used is not None else offset) if ctx.needs_input_grad[0] else None
+        return dx, (dy if ctx.needs_input_grad[1] else None), None, None, None
+
+
+def counter_dropout(x, p, seed, offset=0, residual=None):
+    """Dropout whose mask is a function of (``seed``, ``offset``, element): element e (in the logical order of x) stays
+    when its 16-bit value of Philox4x32-10 is at least round(65536 p), and is scaled by the inverse of the exact
+    probability of staying; a dropped element is 0.  ``residual`` is added to the result.
+
+    Calls that must not share a mask take different offsets.  ``offset`` is an integer or an int64 tensor of one element on
+    x's device that the kernel reads when it runs: a captured graph that advances it draws a new mask on every replay
+    (the backward pass keeps the value its forward pass used)."""
+    if _wants_grad(x, residual):
+        return _DropoutFn.apply(x, residual, p, seed, offset)
+    return ops.dropout_forward(x, p, seed, offset, residual)
+
+
+# ------------------------------------------------------------------------------------ group norm
+class _NormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act, p, seed, offset):
+        used = _used_offset(offset) if p > 0 else None
+        y, stats = ops.group_norm_forward(x, groups, weight, bias, eps, act, p, seed, offset, used)
+        ctx.args = (groups, eps, act, p, seed, None if used is not None else offset)
+        ctx.save_for_backward(x, weight, bias, stats, used)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, stats, used = ctx.saved_tensors
+        groups, eps, act, p, seed, offset = ctx.args
+        dx, dw, db = ops.group_norm_backward(x, groups, weight, bias, eps, act, p, seed, used if used is not None else offset,
+                                             stats, dy)
+        return dx, dw, db, None, None, None, None, None, None
+
+
+def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", p=0.0, seed=0, offset=0):
+    """Group norm over [N, C, H, W], activation (``"none"``, ``"relu"``, ``"silu"``) and, for ``p`` > 0, dropout in one
+    pass.  ``weight`` and ``bias``: float32 [C] or None.  x is taken channels last in memory (another layout is copied into
+    it first) and the result is channels last.  ``seed`` and ``offset`` as in counter_dropout; elements are counted in
+    [N, H, W, C] order."""
+    if _wants_grad(x, weight, bias):
+        return _NormFn.apply(x, weight, bias, num_groups, float(eps), act, float(p), seed, offset)
+    return ops.group_norm_forward(x, num_groups, weight, bias, eps, act, p, seed, offset)[0]
+
+
+class GroupNormAct(nn.Module):
+    """group_norm_act with its parameters; ``p``: dropout of the training mode.  The dropout's offset is a buffer that
+    every training pass advances by one on the device, so passes draw different masks, replays of a captured pass too."""
+
+    def __init__(self, num_groups, num_channels, act="none", p=0.0, eps=1e-5, affine=True, seed=0):
+        super().__init__()
+        self.num_groups, self.num_channels, self.act, self.p, self.eps, self.seed = num_groups, num_channels, act, p, eps, seed
+        self.weight = nn.Parameter(torch.ones(num_channels)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(num_channels)) if affine else None
+        self.register_buffer("offset", torch.zeros(1, dtype=torch.int64))
+
+    def forward(self, x):
+        p = self.p if self.training else 0.0
+        y = group_norm_act(x, self.num_groups, self.weight, self.bias, self.eps, self.act, p, self.seed,
+                           self.offset if p > 0 else 0)
+        if p > 0:
+            self.offset.add_(1)
+        return y
+
+
+class CounterDropout(nn.Module):
+    """counter_dropout in training mode, the identity (plus ``residual``) otherwise; the offset as in GroupNormAct."""
+
+    def __init__(self, p, seed=0):
+        super().__init__()
+        self.p, self.seed = p, seed
+        self.register_buffer("offset", torch.zeros(1, dtype=torch.int64))
+
+    def forward(self, x, residual=None):
+        if not self.training or self.p == 0:
+            return x if residual is None else x + residual
+        y = counter_dropout(x, self.p, self.seed, self.offset, residual)
+        self.offset.add_(1)
+        return y

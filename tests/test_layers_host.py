@@ -1,0 +1,147 @@
+"""The layer operators without a GPU: what the Python entry points and the C ABI refuse before anything is launched."""
+import ctypes as C
+import os
+
+import pytest
+import torch
+
+
+def test_cpu_tensors_are_refused():
+    from pl_convlstm_gan_amd import layers
+    x = torch.zeros(2, 3, 4)
+    for call in (lambda: layers.gated_linear_scan(x, x), lambda: layers.gated_linear_step(x, x, x), lambda: layers.counter_dropout(x, 0.5, 1),
+                 lambda: layers.group_norm_act(x[None], 2), lambda: layers.gated_linear_scan(x.requires_grad_(), x)):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
+    with pytest.raises(TypeError):
+        layers.gated_linear_scan([1.0], x)
+
+
+def scan_desc(**kw):
+    from pl_convlstm_gan_amd import _lib
+    d = _lib.ScanDesc()
+    d.B, d.T, d.D, d.dtype = 2, 40, 8, 0
+    d.x = d.f = d.y = d.h_last = d.dy = d.dx = d.df = d.states = 4096      # (addresses that no launch ever sees)
+    for t in ("x", "f", "dy"):
+        setattr(d, t + "_batch", 320)
+        setattr(d, t + "_step", 8)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def norm_desc(**kw):
+    from pl_convlstm_gan_amd import _lib
+    d = _lib.NormDesc()
+    d.N, d.C, d.G, d.HW, d.dtype, d.eps = 2, 16, 4, 30, 1, 1e-5
+    d.x = d.y = d.stats = d.dy = d.dx = d.workspace = 4096
+    d.workspace_bytes = 1 << 20
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def refused(rc, code, text):
+    from pl_convlstm_gan_amd import _lib
+    msg = _lib.lib().plc_last_error().decode()
+    assert rc == code and text in msg, (rc, msg)
+
+
+def test_scan_abi_refusals():
+    from pl_convlstm_gan_amd import _lib
+    L = _lib.lib()
+    refused(L.plc_gated_scan_fwd(None, None), -1, "null descriptor")
+    for kw, text in ((dict(dtype=9), "element type"), (dict(B=-1), "negative"), (dict(T=-1), "negative"), (dict(D=-1), "negative"),
+                     (dict(x=None), "null input"), (dict(f=None), "null input"), (dict(y=None), "null output"), (dict(x=4098), "misaligned"),
+                     (dict(h0=4098), "misaligned"), (dict(h_last=4097), "misaligned")):
+        refused(L.plc_gated_scan_fwd(C.byref(scan_desc(**kw)), None), -1, text)
+    for kw, text in ((dict(dy=None), "null output"), (dict(dx=None), "null output"), (dict(df=None), "null output"), (dict(states=None), "states"),
+                     (dict(dy=4098), "misaligned"), (dict(dh_last=4099), "misaligned")):
+        refused(L.plc_gated_scan_bwd(C.byref(scan_desc(**kw)), None), -1, text)
+    refused(L.plc_gated_scan_fwd(C.byref(scan_desc(B=1 << 30, D=1 << 20)), None), -2, "one launch")
+    # nothing to do is no error
+    assert L.plc_gated_scan_fwd(C.byref(scan_desc(B=0, x=None, f=None, y=None)), None) == 0
+    assert L.plc_gated_scan_states_bytes(2, 16, 8) == 0 and L.plc_gated_scan_states_bytes(2, 33, 8) == 2 * 2 * 8 * 4
+    assert L.plc_gated_scan_states_bytes(0, 33, 8) == 0
+
+
+def test_norm_abi_refusals():
+    from pl_convlstm_gan_amd import _lib
+    L = _lib.lib()
+    refused(L.plc_group_norm_fwd(None, None), -1, "null descriptor")
+    for kw, text in ((dict(dtype=3), "element type"), (dict(N=-1), "bad size"), (dict(C=0), "bad size"), (dict(G=3), "do not divide"), (dict(G=0), "do not divide"),
+                     (dict(act=3), "activation"), (dict(layout=2), "layout"), (dict(layout=1, C=12), "whole blocks"), (dict(layout=1, x=4098), "16-byte"),
+                     (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(p=2.0), "probability"), (dict(p=float("nan")), "probability"),
+                     (dict(x=4097), "misaligned"), (dict(weight=4098), "misaligned"), (dict(x=None), "null tensor"), (dict(y=None), "null tensor"),
+                     (dict(stats=None), "null tensor"), (dict(workspace=None), "null workspace")):
+        refused(L.plc_group_norm_fwd(C.byref(norm_desc(**kw)), None), -1, text)
+    refused(L.plc_group_norm_bwd(C.byref(norm_desc(dy=None)), None), -1, "null tensor")
+    refused(L.plc_group_norm_fwd(C.byref(norm_desc(workspace_bytes=1)), None), -3, "workspace")
+    refused(L.plc_group_norm_fwd(C.byref(norm_desc(N=(1 << 31) - 1, workspace_bytes=1 << 50)), None), -2, "one launch")
+    need = L.plc_group_norm_workspace_bytes(C.byref(norm_desc()))
+    assert need > 0 and L.plc_group_norm_workspace_bytes(C.byref(norm_desc(G=5))) == 0
+    assert L.plc_group_norm_fwd(C.byref(norm_desc(N=0, x=None, y=None)), None) == 0
+
+
+def test_dropout_abi_refusals():
+    from pl_convlstm_gan_amd import _lib
+    L = _lib.lib()
+    call = lambda x=4096, r=None, y=8192, n=100, dtype=0, p=0.5: L.plc_dropout(x, r, y, n, dtype, p, 1, 2, None, None, None)  # noqa: E731
+    for kw, text in ((dict(dtype=5), "element type"), (dict(n=-1), "negative"), (dict(p=-0.1), "probability"), (dict(p=1.1), "probability"),
+                     (dict(p=float("nan")), "probability"), (dict(x=None), "null"), (dict(y=None), "null"), (dict(x=4098), "misaligned"), (dict(r=4097), "misaligned")):
+        refused(call(**kw), -1, text)
+    refused(call(n=1 << 45), -2, "one launch")
+    assert call(n=0, x=None, y=None) == 0
+
+
+def test_descriptors_mirror_the_header(tmp_path):
+    """Sizes and offsets of the structures as the C compiler lays them out."""
+    import re
+    import shutil
+    import subprocess
+    from conftest import ROOT
+    from pl_convlstm_gan_amd import _lib
+    if not shutil.which("gcc"):
+        pytest.skip("no C compiler")
+    pairs = (("plc_scan_desc", _lib.ScanDesc), ("plc_norm_desc", _lib.NormDesc))
+    lines = []
+    for name, mirror in pairs:
+        lines.append(f'printf("%zu\\n", sizeof({name}));')
+        lines += [f'printf("%zu\\n", offsetof({name}, {f[0]}));' for f in mirror._fields_]
+    src = tmp_path / "t.c"
+    src.write_text('#include <stdio.h>\n#include "%s"\nint main(void) { %s return 0; }\n' % (os.path.join(ROOT, "include", "plconvlstm.h"), " ".join(lines)))
+    subprocess.run(["gcc", "-o", str(tmp_path / "t"), str(src)], check=True)
+    got = [int(v) for v in re.findall(r"\d+", subprocess.run([str(tmp_path / "t")], capture_output=True, text=True, check=True).stdout)]
+    want = []
+    for _, mirror in pairs:
+        want.append(C.sizeof(mirror))
+        want += [getattr(mirror, f[0]).offset for f in mirror._fields_]
+    assert got == want
+
+
+def test_no_packed_fp32_in_any_code_object(tmp_path):
+    """Every device code object of the built library (one per translation unit) is free of packed fp32 arithmetic, which is
+    unreliable on the MI355X beside an MFMA kernel (pl_convlstm_gan_amd/build.py)."""
+    import re
+    import shutil
+    import subprocess
+    from pl_convlstm_gan_amd import _lib
+    llvm = "/opt/rocm/lib/llvm/bin"
+    bundler, objdump = os.path.join(llvm, "clang-offload-bundler"), os.path.join(llvm, "llvm-objdump")
+    objcopy = shutil.which("objcopy")
+    if not (os.path.exists(_lib.LIB_PATH) and os.path.exists(bundler) and os.path.exists(objdump) and objcopy):
+        pytest.skip("library or binary tools not available")
+    fat = tmp_path / "fat.bin"
+    subprocess.run([objcopy, "-O", "binary", "--only-section=.hip_fatbin", _lib.LIB_PATH, str(fat)], check=True)
+    blob = fat.read_bytes()
+    starts = [m.start() for m in re.finditer(b"__CLANG_OFFLOAD_BUNDLE__", blob)]
+    names = ""
+    for k, at in enumerate(starts):
+        piece, co = tmp_path / f"{k}.fat", tmp_path / f"{k}.co"
+        piece.write_bytes(blob[at:(starts + [len(blob)])[k + 1]])
+        subprocess.run([bundler, "--unbundle", "--type=o", f"--input={piece}", "--targets=hipv4-amdgcn-amd-amdhsa--gfx950",
+                        f"--output={co}"], check=True)
+        dis = subprocess.run([objdump, "-d", str(co)], check=True, capture_output=True, text=True).stdout
+        names += dis
+        assert not re.search(r"\bv_pk_(fma|mul|add)_f32\b", dis)
+    assert "plc_scan_fwd_kernel" in names and "plc_lstm_pair_kernel" in names
