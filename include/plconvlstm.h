@@ -412,7 +412,7 @@ enum { PLC_F32 = 0, PLC_BF16 = 1, PLC_F16 = 2 };
  *            are 0, whatever x, f and dy hold there, and the state stands still (h_last of a sample without a step is h0).
  *   h0       NULL = zeros;  h_last NULL = not wanted, else it may be h0 itself (a state updated in place)
  *   states   forward: NULL, or room for plc_gated_scan_states_bytes(B, T, D) bytes that the backward pass reads
- *            (the fp32 state in front of every 16th step; none for T <= 16, where NULL serves the backward pass too)
+ *            (the fp32 state in front of every 8th step; none for T <= 8, where NULL serves the backward pass too)
  * Backward (dh_last, dh0 may be NULL): g_t = dy_t + s_{t+1} g_{t+1}, g behind the last step = dh_last;
  *   coupled: dx_t = (1 - s_t) g_t, df_t = g_t (h_{t-1} - x_t) s_t (1 - s_t);  else dx_t = g_t, df_t = g_t h_{t-1} s_t (1 - s_t);
  *   dh0 = s_0 g_0.  The states are rebuilt in fp32 from x, f and `states`; y is not read.
@@ -461,8 +461,8 @@ int plc_dropout(const void* x, const void* residual, void* y, long long n, int d
 /* Group norm over the HW pixels and C / G channels of each group of each of N samples, with an activation and, when
  * p > 0, dropout in the same pass:
  *   xh = (x - mean) / sqrt(var + eps);  z = weight_c xh + bias_c;  y = dropout(act(z))
- * layout: PLC_NHWC = [N][HW][C], PLC_CB8 = [N][C/8][HW][8] (the engine's activations; C a multiple of 8).  Dropout
- * counts elements in [N][HW][C] order in both.
+ * layout: PLC_NHWC = [N][HW][C], PLC_CB8 = [N][C/8][HW][8] (the engine's activations; C a multiple of 8, 16-bit
+ * elements).  Dropout counts elements in [N][HW][C] order in both.
  *   weight, bias  fp32 [C] or NULL (1, 0);  stats: fp32 [N][G][2] (mean, 1 / sqrt(var + eps)), written by the forward
  *                 and read by the backward pass
  *   dweight, dbias  fp32 [C] or NULL, overwritten
@@ -488,12 +488,12 @@ typedef struct plc_norm_desc {
     void* dx;
     float* dweight;
     float* dbias;
-    /* plc_group_norm_workspace_bytes(desc) bytes, 16-byte aligned */
+    /* plc_group_norm_workspace_bytes(desc, backward) bytes, 16-byte aligned */
     void* workspace;
     size_t workspace_bytes;
 } plc_norm_desc;
 
-size_t plc_group_norm_workspace_bytes(const plc_norm_desc* d);
+size_t plc_group_norm_workspace_bytes(const plc_norm_desc* d, int backward);
 int plc_group_norm_fwd(const plc_norm_desc* d, void* stream);
 int plc_group_norm_bwd(const plc_norm_desc* d, void* stream);
 

@@ -206,7 +206,7 @@ def lib():
     L.plc_dropout.restype = i
     L.plc_dropout.argtypes = [p, p, p, C.c_longlong, i, C.c_double, C.c_ulonglong, C.c_ulonglong, p, p, p]
     L.plc_group_norm_workspace_bytes.restype = sz
-    L.plc_group_norm_workspace_bytes.argtypes = [C.POINTER(NormDesc)]
+    L.plc_group_norm_workspace_bytes.argtypes = [C.POINTER(NormDesc), i]
     for name, desc in (("plc_gated_scan_fwd", ScanDesc), ("plc_gated_scan_bwd", ScanDesc),
                        ("plc_group_norm_fwd", NormDesc), ("plc_group_norm_bwd", NormDesc)):
         fn = getattr(L, name)

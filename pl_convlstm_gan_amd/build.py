@@ -6,8 +6,8 @@ import os
 import subprocess
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-# (the rollout engine, then the layer operators: two translation units, compiled side by side)
-SRCS = [os.path.join(HERE, "csrc", "plc_api.hip"), os.path.join(HERE, "csrc", "plc_layers.hip")]
+# (the rollout engine, the layer operators, and the group norm's kernels by element type: compiled side by side)
+SRCS = [os.path.join(HERE, "csrc", name + ".hip") for name in ("plc_api", "plc_layers", "plc_norm_f32", "plc_norm_bf16", "plc_norm_f16")]
 OUT = os.path.join(HERE, "libplconvlstm.so")
 DEPS = sorted(glob.glob(os.path.join(HERE, "csrc", "*.h")) + glob.glob(os.path.join(HERE, "csrc", "*.hip"))) + \
        [os.path.join(os.path.dirname(HERE), "include", "plconvlstm.h"), os.path.abspath(__file__)]

@@ -30,8 +30,8 @@ __global__ __launch_bounds__(256) void plc_dropout_kernel(DropoutArgs a) {
         float o[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            o[i] = (keep >> i) & 1 ? (float)v.e[i] * d.scale : 0.0f;
-            if (r) o[i] += (float)w.e[i];
+            o[i] = (keep >> i) & 1 ? v.get(i) * d.scale : 0.0f;
+            if (r) o[i] += w.get(i);
         }
         plc_store<T, 8>(y, plc_from_float<T, 8>(o));
     } else {

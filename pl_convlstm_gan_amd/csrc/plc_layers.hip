@@ -6,7 +6,7 @@
 
 #include "plc_host.h"
 #include "plc_dropout_kernels.h"
-#include "plc_norm_kernels.h"
+#include "plc_norm_launch.h"
 #include "plc_scan_kernels.h"
 
 static int dtype_size(int dtype) { return dtype == PLC_F32 ? 4 : (dtype == PLC_BF16 || dtype == PLC_F16 ? 2 : 0); }
@@ -77,12 +77,6 @@ extern "C" size_t plc_gated_scan_states_bytes(int B, int T, long long D) {
     return (size_t)B * ((T + SCAN_K - 1) / SCAN_K - 1) * (size_t)D * 4;
 }
 
-extern "C" size_t plc_gated_scan_workspace_bytes(const plc_scan_desc* d, int backward) {
-    (void)d;
-    (void)backward;
-    return 0;
-}
-
 static int scan_check(const plc_scan_desc* d, bool backward, ScanArgs* a, int* v) {
     PLC_REQUIRE(d, "gated scan: null descriptor");
     const int e = dtype_size(d->dtype);
@@ -117,23 +111,71 @@ static int scan_check(const plc_scan_desc* d, bool backward, ScanArgs* a, int* v
     return PLC_OK;
 }
 
-template <class T>
-static int scan_launch(const ScanArgs& a, bool backward, int v, hipStream_t st) {
-    const long long lanes = a.B * (a.D / v), blocks = (lanes + 255) / 256;
-    if (!grid_ok(blocks, 256)) return plc_fail(PLC_EUNSUPPORTED, "gated scan: %lld lanes are more than one launch covers", lanes);
-    const dim3 grid((unsigned)blocks), block(256);
-#define CALL(V)                                                                                  \
-    if (backward) hipLaunchKernelGGL((plc_scan_bwd_kernel<T, V>), grid, block, 0, st, a);        \
-    else hipLaunchKernelGGL((plc_scan_fwd_kernel<T, V>), grid, block, 0, st, a)
-    switch (v) {
-        case 8: if constexpr (sizeof(T) == 2) { CALL(8); } break;
-        case 4: CALL(4); break;
-        case 2: CALL(2); break;
-        default: CALL(1); break;
+// How a call runs: channels per lane, and segments of time (1: one lane walks the whole sequence).
+static void scan_plan(ScanArgs* a, int vmax, bool backward, int* v) {
+    const long long n = (long long)a->B * a->D;
+    *v = vmax < 4 ? vmax : 4;
+    a->nseg = 1;
+    a->seg = a->T;
+    if (n / *v / 64 < 512 && a->T >= 4 * SCAN_K) {
+        *v = vmax;
+        while (*v > 1 && n / *v < 1024) *v /= 2;
+        const long long tiles = (n / *v + 63) / 64;
+        long long want = 2048 / tiles, most = 512;
+        want = want > most ? most : (want < 1 ? 1 : want);
+        long long seg = (a->T + want - 1) / want;
+        seg = (seg + SCAN_K - 1) / SCAN_K * SCAN_K;
+        a->seg = (int)seg;
+        a->nseg = (int)((a->T + seg - 1) / seg);
+    } else if (vmax == 8 && !backward && n / 8 / 64 >= 4096) {
+        *v = 8;
+    } else {
+        while (*v > 1 && n / *v / 64 < 1024) *v /= 2;
     }
-#undef CALL
+}
+
+template <class T, int V, bool COUPLED, bool BACKWARD>
+static int scan_launch(const ScanArgs& a, hipStream_t st) {
+    const long long lanes = a.B * (a.D / V);
+    if (a.nseg > 1) {
+        const long long blocks = (lanes + 63) / 64 * cdiv(a.nseg, SCAN_WAVES);
+        const dim3 grid((unsigned)blocks), block(64 * SCAN_WAVES);
+        hipLaunchKernelGGL((plc_scan_segments_kernel<T, V, COUPLED, BACKWARD>), grid, block, 0, st, a);
+        hipLaunchKernelGGL((plc_scan_split_kernel<T, V, COUPLED, BACKWARD>), grid, block, 0, st, a);
+    } else {
+        const long long blocks = (lanes + 255) / 256;
+        if (!grid_ok(blocks, 256)) return plc_fail(PLC_EUNSUPPORTED, "gated scan: %lld lanes are more than one launch covers", lanes);
+        const dim3 grid((unsigned)blocks), block(256);
+        if (BACKWARD) hipLaunchKernelGGL((plc_scan_bwd_kernel<T, V, COUPLED>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((plc_scan_fwd_kernel<T, V, COUPLED>), grid, block, 0, st, a);
+    }
     PLC_HIP(hipGetLastError());
     return PLC_OK;
+}
+
+static size_t scan_workspace(const ScanArgs& a) { return a.nseg > 1 ? (size_t)a.nseg * 2 * a.B * (size_t)a.D * 4 : 0; }
+
+extern "C" size_t plc_gated_scan_workspace_bytes(const plc_scan_desc* d, int backward) {
+    ScanArgs a;
+    int v = 1;
+    if (scan_check(d, backward != 0, &a, &v) || a.B == 0 || a.D == 0) return 0;
+    scan_plan(&a, v, backward != 0, &v);
+    return scan_workspace(a);
+}
+
+template <class T, int V>
+static int scan_pick(const ScanArgs& a, bool backward, hipStream_t st) {
+    if (a.coupled) return backward ? scan_launch<T, V, true, true>(a, st) : scan_launch<T, V, true, false>(a, st);
+    return backward ? scan_launch<T, V, false, true>(a, st) : scan_launch<T, V, false, false>(a, st);
+}
+template <class T>
+static int scan_type(const ScanArgs& a, bool backward, int v, hipStream_t st) {
+    switch (v) {
+        case 8: if constexpr (sizeof(T) == 2) return scan_pick<T, 8>(a, backward, st);
+        case 4: return scan_pick<T, 4>(a, backward, st);
+        case 2: return scan_pick<T, 2>(a, backward, st);
+        default: return scan_pick<T, 1>(a, backward, st);
+    }
 }
 
 static int scan_run(const plc_scan_desc* d, bool backward, void* stream) {
@@ -141,12 +183,18 @@ static int scan_run(const plc_scan_desc* d, bool backward, void* stream) {
     int v = 1;
     const int rc = scan_check(d, backward, &a, &v);
     if (rc || a.B == 0 || a.D == 0) return rc;
-    // (four channels at most: with eight, the sixteen steps a lane holds in registers exceed them)
-    if (v > 4) v = 4;
+    scan_plan(&a, v, backward, &v);
+    const size_t need = scan_workspace(a);
+    if (need) {
+        if (!d->workspace || d->workspace_bytes < need)
+            return plc_fail(PLC_EWORKSPACE, "gated scan: workspace %zu < %zu bytes", d->workspace ? d->workspace_bytes : 0, need);
+        PLC_REQUIRE(aligned16(d->workspace), "gated scan: workspace must be 16-byte aligned");
+        a.agg = (float*)d->workspace;
+    }
     switch (d->dtype) {
-        case PLC_F32: return scan_launch<float>(a, backward, v, (hipStream_t)stream);
-        case PLC_BF16: return scan_launch<plc_bf16>(a, backward, v, (hipStream_t)stream);
-        default: return scan_launch<plc_f16>(a, backward, v, (hipStream_t)stream);
+        case PLC_F32: return scan_type<float>(a, backward, v, (hipStream_t)stream);
+        case PLC_BF16: return scan_type<plc_bf16>(a, backward, v, (hipStream_t)stream);
+        default: return scan_type<plc_f16>(a, backward, v, (hipStream_t)stream);
     }
 }
 
@@ -156,7 +204,9 @@ extern "C" int plc_gated_scan_bwd(const plc_scan_desc* d, void* stream) { return
 // ---------------------------------------------------------------------------------------------
 // group norm with an activation
 // ---------------------------------------------------------------------------------------------
-static int norm_geometry(const plc_norm_desc* d, NormArgs* a, int* v) {
+static int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
+
+static int norm_plan(const plc_norm_desc* d, bool backward, NormArgs* a, NormPlan* pl) {
     PLC_REQUIRE(d, "group norm: null descriptor");
     const int e = dtype_size(d->dtype);
     PLC_REQUIRE(e, "group norm: unknown element type %d", d->dtype);
@@ -165,94 +215,111 @@ static int norm_geometry(const plc_norm_desc* d, NormArgs* a, int* v) {
     PLC_REQUIRE(d->act >= PLC_ACT_NONE && d->act <= PLC_ACT_SILU, "group norm: unknown activation %d", d->act);
     PLC_REQUIRE(d->layout == PLC_NHWC || d->layout == PLC_CB8, "group norm: unknown layout %d", d->layout);
     PLC_REQUIRE(d->layout == PLC_NHWC || d->C % 8 == 0, "group norm: the CB8 layout takes whole blocks of 8 channels, not %d", d->C);
+    PLC_REQUIRE(d->layout == PLC_NHWC || e == 2, "group norm: the CB8 layout holds 16-bit elements");
     PLC_REQUIRE(d->eps >= 0.0f, "group norm: negative eps");
     PLC_REQUIRE(d->p >= 0.0 && d->p <= 1.0, "group norm: p = %g is not a probability", d->p);
-    memset(a, 0, sizeof(*a));
-    a->N = d->N; a->C = d->C; a->G = d->G; a->HW = d->HW;
-    a->cg = d->C / d->G;
-    VecRule r{8};
-    r.stride(d->C);
     const void* types[] = {d->x, d->y, d->dy, d->dx};
     for (const void* p : types) PLC_REQUIRE(((uintptr_t)p & (e - 1)) == 0, "group norm: misaligned tensor pointer");
+    memset(a, 0, sizeof(*a));
+    memset(pl, 0, sizeof(*pl));
+    a->N = d->N; a->C = d->C; a->G = d->G; a->HW = d->HW;
+    a->cg = d->C / d->G;
+    VecRule r{16 / e};
+    r.stride(d->C);
     for (const void* p : types) r.pointer(p, e);
     PLC_REQUIRE(d->layout == PLC_NHWC || r.v == 8, "group norm: CB8 tensors must be 16-byte aligned");
-    *v = r.v;
-    a->U = d->C / r.v;
-    a->img = (long long)d->HW * d->C;
-    if (d->layout == PLC_NHWC) {
-        a->us = r.v;
-        a->ps = d->C;
-        a->ut = a->U < 256 ? a->U : 256;
-    } else {
-        a->us = 8ll * d->HW;
-        a->ps = 8;
-        a->ut = 1;
+    int v = r.v;
+    if (e == 4 && v == 2) v = 1;       // (fp32 is compiled for 4 and 1)
+    // the smallest run of units that holds whole groups; a group of more than 256 units is taken in parts, for which a
+    // unit has to lie within one group
+    int m0 = a->cg / gcd(v, a->cg);
+    a->parts = 1;
+    if (m0 > 256) {
+        if (d->layout == PLC_NHWC) v = gcd(v, a->cg);
+        if (e == 4 && v == 2) v = 1;
+        PLC_REQUIRE(a->cg % v == 0, "group norm: CB8 groups of more than 2048 channels must be whole blocks");
+        m0 = a->cg / v;
+        a->gu = m0;
+        a->parts = cdiv(m0, 256);
     }
-    a->tiles = cdiv(a->U, a->ut);
-    const int rows = 256 / a->ut;
-    // pixel ranges: enough workgroups for the chip, at least one round of loads each, at most 64 partial sums for the
-    // second pass to add
-    const long long want = 2048, per = (long long)d->N * a->tiles;
-    long long s = per > 0 ? (want + per - 1) / per : 1;
-    const long long most = d->HW > 0 ? (d->HW + NORM_P * rows - 1) / (NORM_P * rows) : 1;
-    s = s > most ? most : s;
-    s = s > 64 ? 64 : (s < 1 ? 1 : s);
-    a->px_split = d->HW > 0 ? (int)((d->HW + s - 1) / s) : 1;
-    a->splits = d->HW > 0 ? cdiv(d->HW, a->px_split) : 1;
-    a->px_chunk = a->px_split;
-    a->chunks = a->splits;
+    pl->v = v;
+    a->U = d->C / v;
+    a->img = (long long)d->HW * d->C;
+    a->px_first = d->layout == PLC_CB8;
+    a->us = a->px_first ? 8ll * d->HW : v;
+    a->ps = a->px_first ? 8 : d->C;
+    a->splits = 1;
+    a->px_split = d->HW;
+    // Resident form, where the chip is full of tiles of at most four units a thread (rows of up to 128 bytes as long as they
+    // leave 256 tiles), or of larger ones that are many.
+    const int ku_max = backward ? 8 : 16;
+    if (a->parts == 1 && m0 <= 64 && d->HW > 0 && (long long)d->HW * m0 <= 512ll * ku_max) {
+        int widest = m0;
+        if (!a->px_first)
+            while (a->U % (widest * 2) == 0 && widest * v * e < 128) widest *= 2;
+        for (int limit = 4; limit <= ku_max && !pl->ku; limit = limit == 4 ? ku_max : 2 * ku_max)
+            for (int ut = widest; ut >= m0; ut /= 2) {
+                const int need = cdiv(d->HW, 512 / ut);
+                const long long tiles = (long long)d->N * (a->U / ut);
+                if (need > limit || !(tiles >= (limit == 4 ? 256 : 512) || (limit == 4 && ut / 2 < m0))) continue;
+                a->ut = ut;
+                pl->ku = limit;
+                pl->threads = cdiv(d->HW, 256 / ut) <= 4 ? 256 : 512;
+                break;
+            }
+    }
+    if (pl->ku == 0) {
+        // Split form.  NHWC: whole rows up to 256 units; CB8: the smallest tile.
+        if (a->parts > 1) a->ut = cdiv(a->gu, a->parts);
+        else a->ut = a->px_first ? m0 : (a->U < 256 ? a->U : 256 / m0 * m0);
+        pl->threads = 256;
+        const int rows = 256 / a->ut, p = backward ? NORM_PB : NORM_P;
+        a->tiles = a->parts > 1 ? a->G * a->parts : cdiv(a->U, a->ut);
+        // pixel ranges: enough workgroups for the chip, two rounds of loads each at least, at most 64 per sample
+        const long long per = (long long)d->N * a->tiles, want = per > 0 ? (4096 + per - 1) / per : 1;
+        const long long most = d->HW > 0 ? (d->HW + 2 * p * rows - 1) / (2 * p * rows) : 1;
+        long long s = want < most ? want : most;
+        s = s > 256 ? 256 : (s < 1 ? 1 : s);
+        a->px_split = d->HW > 0 ? (int)((d->HW + s - 1) / s) : 1;
+        a->splits = d->HW > 0 ? cdiv(d->HW, a->px_split) : 1;
+    }
+    a->tiles = a->parts > 1 ? a->G * a->parts : cdiv(a->U, a->ut);
     a->act = d->act;
     a->eps = d->eps;
     a->x = d->x; a->dy = d->dy; a->y = d->y; a->dx = d->dx;
     a->w = d->weight; a->b = d->bias; a->dw = d->dweight; a->db = d->dbias;
     a->stats = d->stats;
-    a->part = (float*)d->workspace;
     a->drop = drop_of(d->p, d->seed, d->offset);
     a->offset_ptr = d->offset_ptr;
     a->used_offset = d->used_offset;
+    pl->part_g = 0;
+    pl->part_c = align256((size_t)a->N * a->G * a->splits * a->parts * 2 * sizeof(float));
+    pl->total = pl->part_c + (backward ? (size_t)a->N * a->splits * a->C * 2 * sizeof(float) : 0);
     return PLC_OK;
 }
 
-static size_t norm_workspace(const NormArgs& a) { return (size_t)a.N * a.splits * a.C * 2 * sizeof(float); }
-
-extern "C" size_t plc_group_norm_workspace_bytes(const plc_norm_desc* d) {
+extern "C" size_t plc_group_norm_workspace_bytes(const plc_norm_desc* d, int backward) {
     NormArgs a;
-    int v;
-    if (norm_geometry(d, &a, &v) != PLC_OK) return 0;
-    return norm_workspace(a);
+    NormPlan pl;
+    if (norm_plan(d, backward != 0, &a, &pl) != PLC_OK) return 0;
+    return pl.total;
 }
 
-static int norm_check(const plc_norm_desc* d, bool backward, NormArgs* a, int* v) {
-    const int rc = norm_geometry(d, a, v);
+static int norm_check(const plc_norm_desc* d, bool backward, NormArgs* a, NormPlan* pl) {
+    const int rc = norm_plan(d, backward, a, pl);
     if (rc) return rc;
     const bool any = d->N > 0 && d->HW > 0;
     PLC_REQUIRE(!any || (d->x && d->stats && (backward ? d->dy && d->dx : d->y != nullptr)), "group norm: null tensor pointer");
     PLC_REQUIRE(!any || d->workspace, "group norm: null workspace");
-    PLC_REQUIRE((((uintptr_t)d->weight | (uintptr_t)d->bias | (uintptr_t)d->stats | (uintptr_t)d->workspace |
-                  (uintptr_t)d->dweight | (uintptr_t)d->dbias) & 3) == 0, "group norm: misaligned float pointer");
-    if (any && d->workspace_bytes < norm_workspace(*a))
-        return plc_fail(PLC_EWORKSPACE, "group norm: workspace %zu < %zu bytes", d->workspace_bytes, norm_workspace(*a));
-    const long long blocks = (long long)a->N * a->tiles * (a->splits > a->chunks ? a->splits : a->chunks) + cdiv(a->C, NORM_PARAM_CH);
-    if (!grid_ok(blocks, 256)) return plc_fail(PLC_EUNSUPPORTED, "group norm: %d samples are more than one launch covers", d->N);
-    return PLC_OK;
-}
-
-template <class T, int V>
-static int norm_launch(NormArgs a, bool backward, hipStream_t st) {
-    const unsigned per = (unsigned)a.N * a.tiles;
-    const int nch = a.ut * V;
-    const int sum_lds = (2 * nch + 256 * V * (backward ? 2 : 1)) * (int)sizeof(float);
-    if (!backward) {
-        hipLaunchKernelGGL((plc_norm_stats_kernel<T, V>), dim3(per * a.splits), dim3(256), sum_lds, st, a);
-        hipLaunchKernelGGL((plc_norm_fwd_kernel<T, V>), dim3(per * a.chunks), dim3(256), 2 * (nch + 1) * sizeof(float), st, a);
-    } else {
-        hipLaunchKernelGGL((plc_norm_bwd_sums_kernel<T, V>), dim3(per * a.splits), dim3(256), sum_lds, st, a);
-        a.param_blocks = a.dw || a.db ? cdiv(a.C, NORM_PARAM_CH) : 0;
-        int lds = 4 * (nch + 1) * (int)sizeof(float);
-        if (lds < 2 * 256 * (int)sizeof(double)) lds = 2 * 256 * (int)sizeof(double);
-        hipLaunchKernelGGL((plc_norm_bwd_kernel<T, V>), dim3(per * a.chunks + a.param_blocks), dim3(256), lds, st, a);
-    }
-    PLC_HIP(hipGetLastError());
+    PLC_REQUIRE((((uintptr_t)d->weight | (uintptr_t)d->bias | (uintptr_t)d->stats | (uintptr_t)d->dweight | (uintptr_t)d->dbias) & 3) == 0,
+                "group norm: misaligned float pointer");
+    PLC_REQUIRE(aligned16(d->workspace), "group norm: workspace must be 16-byte aligned");
+    if (any && d->workspace_bytes < pl->total)
+        return plc_fail(PLC_EWORKSPACE, "group norm: workspace %zu < %zu bytes", d->workspace_bytes, pl->total);
+    a->part_g = (float*)((char*)d->workspace + pl->part_g);
+    a->part_c = (float*)((char*)d->workspace + pl->part_c);
+    const long long blocks = (long long)a->N * a->tiles * a->splits + cdiv(a->C, NORM_PARAM_CH);
+    if (!grid_ok(blocks, pl->threads)) return plc_fail(PLC_EUNSUPPORTED, "group norm: %d samples are more than one launch covers", d->N);
     return PLC_OK;
 }
 
@@ -265,8 +332,8 @@ __global__ void plc_norm_clear_kernel(float* a, float* b, int n) {
 
 static int norm_run(const plc_norm_desc* d, bool backward, void* stream) {
     NormArgs a;
-    int v = 1;
-    const int rc = norm_check(d, backward, &a, &v);
+    NormPlan pl;
+    const int rc = norm_check(d, backward, &a, &pl);
     if (rc) return rc;
     hipStream_t st = (hipStream_t)stream;
     if (a.N == 0 || a.HW == 0) {          // no element: the parameters' gradients are sums over nothing
@@ -276,16 +343,11 @@ static int norm_run(const plc_norm_desc* d, bool backward, void* stream) {
         }
         return PLC_OK;
     }
-#define CALL(T)                                             \
-    switch (v) {                                            \
-        case 8: return norm_launch<T, 8>(a, backward, st);  \
-        case 4: return norm_launch<T, 4>(a, backward, st);  \
-        case 2: return norm_launch<T, 2>(a, backward, st);  \
-        default: return norm_launch<T, 1>(a, backward, st); \
+    switch (d->dtype) {
+        case PLC_F32: return plc_norm_launch_f32(a, pl, backward, st);
+        case PLC_BF16: return plc_norm_launch_bf16(a, pl, backward, st);
+        default: return plc_norm_launch_f16(a, pl, backward, st);
     }
-    PLC_BY_TYPE(d->dtype, CALL)
-#undef CALL
-    return PLC_OK;
 }
 
 extern "C" int plc_group_norm_fwd(const plc_norm_desc* d, void* stream) { return norm_run(d, false, stream); }

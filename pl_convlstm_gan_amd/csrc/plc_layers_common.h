@@ -7,10 +7,32 @@
 typedef __bf16 plc_bf16;
 typedef _Float16 plc_f16;
 
-// V consecutive elements of T, moved as one access of V * sizeof(T) bytes (16 at most; wider ones as several)
+template <bool WHOLE>
+struct PlcWord {
+    typedef uint32_t type;
+};
+template <>
+struct PlcWord<false> {
+    typedef unsigned short type;
+};
+
+// V consecutive elements of T, moved as one access of V * sizeof(T) bytes (16 at most; wider ones as several).  They are
+// kept as the words that were loaded and unpacked where they are used: held as separate 16-bit values, each would take a
+// register of its own.
 template <class T, int V>
 struct alignas(V * sizeof(T) > 16 ? 16 : V * sizeof(T)) PlcVec {
-    T e[V];
+    static constexpr int NW = V * sizeof(T) >= 4 ? V * sizeof(T) / 4 : 1;
+    using Word = typename PlcWord<(V * sizeof(T) >= 4)>::type;
+    Word w[NW];
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (sizeof(T) == 4) {
+            return __builtin_bit_cast(float, w[i]);
+        } else {
+            const uint32_t q = (uint32_t)w[i >> 1];
+            if constexpr (__is_same(T, plc_bf16)) return __builtin_bit_cast(float, (i & 1) ? q & 0xffff0000u : q << 16);
+            else return (float)__builtin_bit_cast(plc_f16, (unsigned short)((i & 1) ? q >> 16 : q & 0xffffu));
+        }
+    }
 };
 
 template <class T, int V>
@@ -21,17 +43,29 @@ template <class T, int V>
 __device__ __forceinline__ void plc_store(T* p, const PlcVec<T, V>& v) {
     *reinterpret_cast<PlcVec<T, V>*>(p) = v;
 }
-// (conversions from fp32 round to nearest even: results and gradients leave in the inputs' type, rounded once)
 template <class T, int V>
 __device__ __forceinline__ void plc_to_float(const PlcVec<T, V>& v, float (&o)[V]) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = (float)v.e[i];
+    for (int i = 0; i < V; ++i) o[i] = v.get(i);
 }
+// (conversions from fp32 round to nearest even: results and gradients leave in the inputs' type, rounded once)
 template <class T, int V>
 __device__ __forceinline__ PlcVec<T, V> plc_from_float(const float (&v)[V]) {
     PlcVec<T, V> o;
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) o.e[i] = (T)v[i];
+        for (int i = 0; i < V; ++i) o.w[i] = __builtin_bit_cast(uint32_t, v[i]);
+    } else if constexpr (V == 1) {
+        o.w[0] = __builtin_bit_cast(unsigned short, (T)v[0]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            typedef float F2 __attribute__((ext_vector_type(2)));
+            typedef T T2 __attribute__((ext_vector_type(2)));
+            const F2 f = {v[2 * i], v[2 * i + 1]};
+            o.w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f, T2));
+        }
+    }
     return o;
 }
 

@@ -5,10 +5,14 @@
 //   backward: dz = dy (keep ? scale : 0) act'(z);  db_c = sum dz;  dw_c = sum dz xh;
 //             dx = r (w dz - mean(w dz) - xh mean(w dz xh)), the means over the group
 //
-// A tensor is a set of V-channel units: unit u of pixel p of sample n lies at n * img + u * us + p * ps (elements).
-// That covers [N][HW][C] (us = V, ps = C) and the engine's CB8 ([N][C/8][HW][8]: us = 8 HW, ps = 8).  A workgroup
-// takes `ut` neighbouring units of one sample: NHWC as many as make whole rows, CB8 one plane, so that its lanes read
-// consecutive memory either way.
+// A tensor is a set of V-channel units of at most 16 bytes: unit u of pixel p of sample n lies at n * img + u * us + p * ps
+// (elements).  That covers [N][HW][C] (us = V, ps = C) and the engine's CB8 ([N][C/8][HW][8]: us = 8 HW, ps = 8).
+// A workgroup takes a tile of neighbouring units that holds whole groups (a group wider than a tile: a part of one) and
+// runs with its lanes along the memory's fast direction, units first in NHWC, pixels first in CB8.
+//
+// Two forms.  Resident: the tile's pixels of a sample stay in the registers of one workgroup between the statistics and
+// the output, one launch.  Split: a first launch writes partial sums over ranges of pixels, the second adds them up
+// (every workgroup for its own groups) and makes the output, reading its inputs a second time.
 #pragma once
 #include "plc_layers_common.h"
 
@@ -18,10 +22,12 @@ struct NormArgs {
     int N, C, G, HW;
     int cg;                       // C / G
     int U;                        // units of a sample: C / V
-    int ut;                       // units of a workgroup; rows of threads: blockDim / ut
-    int tiles;                    // workgroups along the units
-    int splits, px_split;         // statistics passes: pixel ranges of a sample and their length
-    int chunks, px_chunk;         // output passes
+    int ut;                       // units of a tile at most
+    int parts;                    // 1: a tile holds whole groups; else: tiles of one group
+    int gu;                       // parts > 1: units of a group
+    int tiles;                    // of a sample
+    int splits, px_split;         // pixel ranges of a sample and their length
+    int px_first;                 // lanes run along pixels (CB8)
     int param_blocks;             // backward output pass: leading workgroups that sum dw and db
     long long img, us, ps;
     int act;
@@ -30,100 +36,289 @@ struct NormArgs {
     const float *w, *b;           // [C] or null (1 and 0)
     void *y, *dx;
     float* stats;                 // [N][G][2]: mean, 1 / sqrt(v + eps)
-    float* part;                  // [N][splits][C][2]: forward mean and sum of squared differences, backward sum dz, dz xh
+    float* part_g;                // [N][G][splits * parts][2]: forward mean and sum of squared differences, backward sums of w dz, w dz xh
+    float* part_c;                // backward: [N * splits][C][2]: sums of dz, dz xh
     float *dw, *db;               // [C] or null
     PlcDrop drop;                 // thr == 0: no dropout
     const long long* offset_ptr;  // device: drop.offset, or null
     long long* used_offset;       // device: receives the offset this call used, or null
 };
 
-// workgroup -> (sample, tile of units, pixel range): one dimension, so that the number of samples is not limited by a
-// grid dimension's 16 bits
+// workgroup -> (sample, tile, pixel range): one dimension, so that the number of samples is not limited by a grid
+// dimension's 16 bits
 struct NormBlock {
-    int n, tile, range;
+    int n, range;
+    int u0, nu;                   // the tile's units
+    int g0, ng;                   // its groups
+    int part;
 };
+template <int V>
 __device__ __forceinline__ NormBlock norm_block(const NormArgs& a, unsigned i, int ranges) {
     NormBlock b;
     const unsigned q = i / (unsigned)ranges;
     b.range = (int)(i - q * (unsigned)ranges);
     b.n = (int)(q / (unsigned)a.tiles);
-    b.tile = (int)(q - (unsigned)b.n * (unsigned)a.tiles);
+    const int tile = (int)(q - (unsigned)b.n * (unsigned)a.tiles);
+    if (a.parts == 1) {
+        b.part = 0;
+        b.u0 = tile * a.ut;
+        b.nu = min(a.ut, a.U - b.u0);
+        b.g0 = b.u0 * V / a.cg;
+        b.ng = b.nu * V / a.cg;
+    } else {
+        b.g0 = tile / a.parts;
+        b.ng = 1;
+        b.part = tile - b.g0 * a.parts;
+        b.u0 = b.g0 * a.gu + b.part * a.ut;
+        b.nu = min(a.ut, a.gu - b.part * a.ut);
+    }
     return b;
 }
 
+// thread -> (unit of the tile, row): a row is one pixel of a round, and threads beyond whole rows are idle
 struct NormTid {
-    int u, r, rows;               // unit within the workgroup, row, number of rows
+    int u, r, rows;
     bool on;
 };
-__device__ __forceinline__ NormTid norm_tid(const NormArgs& a) {
+__device__ __forceinline__ NormTid norm_tid(const NormArgs& a, const NormBlock& b) {
     NormTid t;
-    t.rows = blockDim.x / a.ut;
-    t.u = threadIdx.x % a.ut;
-    t.r = threadIdx.x / a.ut;
-    t.on = t.r < t.rows;
+    t.rows = blockDim.x / b.nu;
+    t.u = a.px_first ? threadIdx.x / t.rows : threadIdx.x % b.nu;
+    t.r = a.px_first ? threadIdx.x % t.rows : threadIdx.x / b.nu;
+    t.on = t.u < b.nu && t.r < t.rows;
     return t;
 }
 
-// Sum over the rows of a workgroup of NV values per channel: every thread brings v[NV][V] of its unit, out[k][ut * V]
-// (LDS) receives the sums.  Fixed order.  scratch: NV * rows * ut * V floats (LDS); ends with a barrier.
+// ---- sums over the rows of a workgroup --------------------------------------------------------------------------
+// Every thread brings NV values per channel of its unit; out[k * nch + channel of the tile] (LDS) receives their sums over
+// the rows, in a fixed order: a thread per (channel, share of the rows), then one per channel.  Scratch: NV * V * (threads +
+// tile units) floats, padded so that the lanes of a wave read different banks.  Begins and ends with a barrier.
 template <int V, int NV>
-__device__ __forceinline__ void norm_sum_rows(const NormTid& t, int ut, const float (&v)[NV][V], float* scratch, float* out) {
-    const int nch = ut * V, n = t.rows * nch;
+__device__ __forceinline__ void norm_sum_rows(const NormTid& t, int nu, const float (&v)[NV][V], float* scratch, float* out) {
+    const int nch = nu * V, pitch = blockDim.x + nu;
+    __syncthreads();
     if (t.on) {
 #pragma unroll
         for (int k = 0; k < NV; ++k)
 #pragma unroll
-            for (int i = 0; i < V; ++i) scratch[k * n + t.r * nch + t.u * V + i] = v[k][i];
+            for (int i = 0; i < V; ++i) scratch[(k * V + i) * pitch + t.r * nu + t.u] = v[k][i];
     }
     __syncthreads();
-    for (int half = t.rows; half > 1;) {
-        const int lower = (half + 1) / 2;
-        for (int i = threadIdx.x; i < (half - lower) * nch; i += blockDim.x)
+    const int shares = max(1, min(t.rows, (int)blockDim.x / nch));
+    float s[NV];
+    for (int base = 0; base < nch * shares; base += blockDim.x) {            // (one round unless the tile has more channels than threads)
+        const int id = base + threadIdx.x, ch = id % nch, share = id / nch;
+        const bool mine = id < nch * shares;
+        const int i = ch / nu, u = ch - i * nu;
 #pragma unroll
-            for (int k = 0; k < NV; ++k) scratch[k * n + i] += scratch[k * n + i + lower * nch];
-        __syncthreads();
-        half = lower;
+        for (int k = 0; k < NV; ++k) s[k] = 0.0f;
+        if (mine)
+#pragma unroll 8
+            for (int r = share; r < t.rows; r += shares)
+#pragma unroll
+                for (int k = 0; k < NV; ++k) s[k] += scratch[(k * V + i) * pitch + r * nu + u];
+        if (shares == 1) {
+            if (mine)
+#pragma unroll
+                for (int k = 0; k < NV; ++k) out[k * nch + u * V + i] = s[k];
+        } else {
+            __syncthreads();
+            if (mine)
+#pragma unroll
+                for (int k = 0; k < NV; ++k) scratch[k * (nch * shares) + id] = s[k];
+            __syncthreads();
+            for (int c = threadIdx.x; c < nch; c += blockDim.x) {
+                const int ci = c / nu, cu = c - ci * nu;
+#pragma unroll
+                for (int k = 0; k < NV; ++k) {
+                    float q = 0.0f;
+#pragma unroll 8
+                    for (int h = 0; h < shares; ++h) q += scratch[k * (nch * shares) + h * nch + c];
+                    out[k * nch + cu * V + ci] = q;
+                }
+            }
+        }
     }
-    for (int i = threadIdx.x; i < nch; i += blockDim.x)
+    __syncthreads();
+}
+// floats of LDS for the above: out and scratch
+__host__ __device__ constexpr int norm_lds_floats(int threads, int nu, int V, int NV) { return NV * nu * V + NV * V * (threads + nu); }
+
+// Sum over the 64 lanes, in every lane.  Lane shifts inside the vector unit: shuffles go through LDS, at about ten times
+// the latency, and every workgroup of the second passes starts with a few of these.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float norm_lane_add(float v) {
+    const int moved = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false);
+    return v + __builtin_bit_cast(float, moved);
+}
+__device__ __forceinline__ float norm_wave_sum(float v) {
+    v = norm_lane_add<0x111, 0xf>(v);      // row_shr:1, 2, 4, 8: lane 15 of each row of 16 has the row's sum
+    v = norm_lane_add<0x112, 0xf>(v);
+    v = norm_lane_add<0x114, 0xf>(v);
+    v = norm_lane_add<0x118, 0xf>(v);
+    v = norm_lane_add<0x142, 0xa>(v);      // row_bcast:15 into rows 1 and 3
+    v = norm_lane_add<0x143, 0xc>(v);      // row_bcast:31 into rows 2 and 3: lane 63 has the sum
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
+// ---- activation -------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float norm_sigmoid(float z) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * z));
+}
+// What a kernel is compiled for: FORM = activation + 3 * dropout, or -1, which asks the arguments for every element (the
+// vector widths that few shapes take).  Compiled in, an element has no branch.
+template <int FORM>
+__device__ __forceinline__ int norm_form_act(const NormArgs& a) { return FORM >= 0 ? FORM % 3 : a.act; }
+template <int FORM>
+__device__ __forceinline__ bool norm_form_drop(const NormArgs& a) { return FORM >= 0 ? FORM >= 3 : a.drop.thr != 0; }
+
+__device__ __forceinline__ float norm_act(float z, int act) {
+    if (act == NORM_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
+    if (act == NORM_ACT_SILU) return z * norm_sigmoid(z);
+    return z;
+}
+// silu'(z)
+__device__ __forceinline__ float norm_silu_slope(float z) {
+    const float s = norm_sigmoid(z);
+    return __builtin_fmaf(z * s, 1.0f - s, s);
+}
+
+template <int FORM>
+__device__ __forceinline__ PlcDrop norm_drop(const NormArgs& a) {
+    PlcDrop d = a.drop;
+    if (norm_form_drop<FORM>(a) && a.offset_ptr) d.offset = (uint64_t)*a.offset_ptr;
+    return d;
+}
+// (elements are counted in [N][HW][C] order whatever the layout, so that one seed gives one mask)
+template <int V>
+__device__ __forceinline__ uint32_t norm_keep(const NormArgs& a, const PlcDrop& d, int n, int p, int u) {
+    return plc_keep_bits<V>(d, ((uint64_t)n * a.HW + p) * a.C + (uint64_t)u * V);
+}
+
+// per-channel constants of a thread's unit.  The difference x - mean is formed first (the mean may be many deviations from
+// 0), r and the weight are one factor.
+template <int V>
+struct NormUnit {
+    float mean[V], r[V], rw[V], b[V];
+};
+template <int V>
+__device__ __forceinline__ void norm_unit(const NormArgs& a, const NormBlock& blk, int u, const float* st, NormUnit<V>& k) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k) out[k * nch + i] = scratch[k * n + i];
+    for (int i = 0; i < V; ++i) {
+        const int c = (blk.u0 + u) * V + i, g = c / a.cg - blk.g0;
+        k.mean[i] = st[2 * g];
+        k.r[i] = st[2 * g + 1];
+        k.rw[i] = k.r[i] * (a.w ? a.w[c] : 1.0f);
+        k.b[i] = a.b ? a.b[c] : 0.0f;
+    }
+}
+
+template <class T, int V, int FORM>
+__device__ __forceinline__ PlcVec<T, V> norm_out(const NormArgs& a, const NormUnit<V>& k, const PlcDrop& drop, int n, int p, int u,
+                                                 const PlcVec<T, V>& x) {
+    const bool drops = norm_form_drop<FORM>(a);
+    const int act = norm_form_act<FORM>(a);
+    const uint32_t keep = drops ? norm_keep<V>(a, drop, n, p, u) : 0;
+    float o[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        o[i] = norm_act(__builtin_fmaf(x.get(i) - k.mean[i], k.rw[i], k.b[i]), act);
+        if (drops) o[i] = (keep >> i) & 1 ? o[i] * drop.scale : 0.0f;
+    }
+    return plc_from_float<T, V>(o);
+}
+
+// d = x - mean and dz of one unit
+template <class T, int V, int FORM>
+__device__ __forceinline__ void norm_dz(const NormArgs& a, const NormUnit<V>& k, const PlcDrop& drop, int n, int p, int u,
+                                        const PlcVec<T, V>& xr, const PlcVec<T, V>& gr, float (&d)[V], float (&dz)[V]) {
+    const bool drops = norm_form_drop<FORM>(a);
+    const int act = norm_form_act<FORM>(a);
+    const uint32_t keep = drops ? norm_keep<V>(a, drop, n, p, u) : 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        d[i] = xr.get(i) - k.mean[i];
+        const float z = __builtin_fmaf(d[i], k.rw[i], k.b[i]), g = gr.get(i);
+        if (act == NORM_ACT_RELU) dz[i] = z > 0.0f ? g : 0.0f;
+        else if (act == NORM_ACT_SILU) dz[i] = g * norm_silu_slope(z);
+        else dz[i] = g;
+        if (drops) dz[i] = (keep >> i) & 1 ? dz[i] * drop.scale : 0.0f;
+    }
+}
+
+__device__ __forceinline__ void norm_load_stats(const NormArgs& a, const NormBlock& blk, float* st) {
+    for (int i = threadIdx.x; i < 2 * blk.ng; i += blockDim.x) st[i] = a.stats[((long long)blk.n * a.G + blk.g0) * 2 + i];
     __syncthreads();
 }
 
-// ---- forward, first pass: per channel of a pixel range, mean and sum of squared differences from it ------------
-// Blocks of NORM_P pixels are reduced around their own mean and merged by the parallel form of the variance
-// (Chan, Golub, LeVeque 1983): sums of squares around 0 would cancel where the mean is far from 0.
-constexpr int NORM_P = 4;
+// Calls f(first pixel, number of pixels, loaded units) for rounds of P pixels of a thread; whole rounds carry no conditions,
+// so that all their loads are in flight at once.
+template <class T, int V, int P, int NT, class F>
+__device__ __forceinline__ void norm_rounds(const T* const (&src)[NT], long long ps, int p0, int p1, int rows, F f) {
+    PlcVec<T, V> raw[NT][P];
+    int p = p0;
+    for (; p + (P - 1) * rows < p1; p += P * rows) {
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+#pragma unroll
+            for (int k = 0; k < NT; ++k) raw[k][j] = plc_load<T, V>(src[k] + (long long)(p + j * rows) * ps);
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            PlcVec<T, V> one[NT];
+#pragma unroll
+            for (int k = 0; k < NT; ++k) one[k] = raw[k][j];
+            f(p + j * rows, one);
+            // (pixel by pixel: left alone, the compiler works on all of them at once, at twice the registers)
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    if (p < p1) {
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+            if (p + j * rows < p1) {
+#pragma unroll
+                for (int k = 0; k < NT; ++k) raw[k][j] = plc_load<T, V>(src[k] + (long long)(p + j * rows) * ps);
+            }
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+            if (p + j * rows < p1) {
+                PlcVec<T, V> one[NT];
+#pragma unroll
+                for (int k = 0; k < NT; ++k) one[k] = raw[k][j];
+                f(p + j * rows, one);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+    }
+}
+
+// ---- split form, forward, first pass ----------------------------------------------------------------------------
+// Per channel of a pixel range, mean and sum of squared differences from it: blocks of NORM_P pixels are reduced around
+// their own mean and merged by the parallel form of the variance (Chan, Golub, LeVeque 1983), since sums of squares around 0
+// would cancel where the mean is far from 0.  The channels of a group are merged the same way at the end.
+constexpr int NORM_P = 8;             // pixels a thread has in flight (forward); half of it for two tensors
 
 template <class T, int V>
 __global__ __launch_bounds__(256) void plc_norm_stats_kernel(NormArgs a) {
     extern __shared__ __align__(16) float lds[];
-    const NormTid t = norm_tid(a);
-    const NormBlock blk = norm_block(a, blockIdx.x, a.splits);
-    const int n = blk.n, u0 = blk.tile * a.ut;
-    const int nu = a.U - u0 < a.ut ? a.U - u0 : a.ut;
-    const int p0 = blk.range * a.px_split, p1 = p0 + a.px_split < a.HW ? p0 + a.px_split : a.HW;
-    const T* x = (const T*)a.x + n * a.img + (long long)(u0 + t.u) * a.us;
+    const NormBlock blk = norm_block<V>(a, blockIdx.x, a.splits);
+    const NormTid t = norm_tid(a, blk);
+    const int p0 = blk.range * a.px_split, p1 = min(p0 + a.px_split, a.HW);
+    const T* x = (const T*)a.x + blk.n * a.img + (long long)(blk.u0 + t.u) * a.us;
     float mean[V], m2[V], count = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) mean[i] = m2[i] = 0.0f;
-    if (t.on && t.u < nu) {
-        for (int p = p0 + t.r; p < p1; p += NORM_P * t.rows) {
-            PlcVec<T, V> raw[NORM_P];
-#pragma unroll
-            for (int j = 0; j < NORM_P; ++j)
-                if (p + j * t.rows < p1) raw[j] = plc_load<T, V>(x + (long long)(p + j * t.rows) * a.ps);
-            const int m = min(NORM_P, (p1 - p + t.rows - 1) / t.rows);
-            const float inv = 1.0f / (float)m, frac = (float)m / (count + (float)m), cross = count * frac;
+    if (t.on) {
+        auto merge = [&](int m, const PlcVec<T, V> (&raw)[NORM_P], bool full) {
+            const float inv = full ? 1.0f / NORM_P : 1.0f / (float)m, frac = (float)m * __builtin_amdgcn_rcpf(count + (float)m), cross = count * frac;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 float s = 0.0f, q = 0.0f;
 #pragma unroll
-                for (int j = 0; j < NORM_P; ++j) s += j < m ? (float)raw[j].e[i] : 0.0f;
+                for (int j = 0; j < NORM_P; ++j) s += full || j < m ? raw[j].get(i) : 0.0f;
                 const float c = s * inv;
 #pragma unroll
                 for (int j = 0; j < NORM_P; ++j) {
-                    const float d = j < m ? (float)raw[j].e[i] - c : 0.0f;
+                    const float d = full || j < m ? raw[j].get(i) - c : 0.0f;
                     q = __builtin_fmaf(d, d, q);
                 }
                 const float delta = c - mean[i];
@@ -131,323 +326,437 @@ __global__ __launch_bounds__(256) void plc_norm_stats_kernel(NormArgs a) {
                 m2[i] += __builtin_fmaf(delta * delta, cross, q);
             }
             count += (float)m;
+        };
+        int p = p0 + t.r;
+        for (; p + (NORM_P - 1) * t.rows < p1; p += NORM_P * t.rows) {
+            PlcVec<T, V> raw[NORM_P];
+#pragma unroll
+            for (int j = 0; j < NORM_P; ++j) raw[j] = plc_load<T, V>(x + (long long)(p + j * t.rows) * a.ps);
+            merge(NORM_P, raw, true);
         }
-    }
-    // the rows of the workgroup: mean = sum n_r mean_r / n, then sum of m2_r + n_r (mean_r - mean)^2
-    const int nch = a.ut * V, total = p1 - p0;
-    float* sums = lds;
-    float* scratch = lds + 2 * nch;
-    float v[1][V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[0][i] = count * mean[i];
-    norm_sum_rows<V, 1>(t, a.ut, v, scratch, sums);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const float d = t.on ? mean[i] - sums[t.u * V + i] / (float)total : 0.0f;
-        v[0][i] = __builtin_fmaf(count * d, d, m2[i]);
-    }
-    norm_sum_rows<V, 1>(t, a.ut, v, scratch, sums + nch);
-    float* part = a.part + (((long long)n * a.splits + blk.range) * a.C + (long long)u0 * V) * 2;
-    for (int i = threadIdx.x; i < nu * V; i += blockDim.x) {
-        part[2 * i] = sums[i] / (float)total;
-        part[2 * i + 1] = sums[nch + i];
-    }
-}
-
-// ---- the groups that a workgroup's channels touch: mean and r from the partials, into LDS -----------------------
-// st[2 g'], g' counted from the first group of the workgroup.  One wave per group, lanes over (split, channel).
-__device__ __forceinline__ float norm_wave_sum(float v) {
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m);
-    return v;
-}
-
-__device__ __forceinline__ void norm_group_stats(const NormArgs& a, int n, int c0, int c1, float* st, bool keep) {
-    const int g0 = c0 / a.cg, g1 = (c1 - 1) / a.cg;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
-    const long long items = (long long)a.splits * a.cg;
-    const float whole = (float)a.px_split, last = (float)(a.HW - (long long)(a.splits - 1) * a.px_split);
-    for (int g = g0 + wave; g <= g1; g += waves) {
-        const float* part = a.part + ((long long)n * a.splits * a.C + (long long)g * a.cg) * 2;
-        float s = 0.0f;
-        for (long long i = lane; i < items; i += 64) {
-            const long long sp = i / a.cg, c = i - sp * a.cg;
-            s = __builtin_fmaf(sp == a.splits - 1 ? last : whole, part[(sp * a.C + c) * 2], s);
-        }
-        const float m = (float)a.HW * (float)a.cg, mean = norm_wave_sum(s) / m;
-        float q = 0.0f;
-        for (long long i = lane; i < items; i += 64) {
-            const long long sp = i / a.cg, c = i - sp * a.cg;
-            const float d = part[(sp * a.C + c) * 2] - mean;
-            q += part[(sp * a.C + c) * 2 + 1] + (sp == a.splits - 1 ? last : whole) * d * d;
-        }
-        const float var = norm_wave_sum(q) / m, r = 1.0f / sqrtf(var + a.eps);
-        if (lane == 0) {
-            st[2 * (g - g0)] = mean;
-            st[2 * (g - g0) + 1] = r;
-            if (keep) {
-                a.stats[((long long)n * a.G + g) * 2] = mean;
-                a.stats[((long long)n * a.G + g) * 2 + 1] = r;
-            }
-        }
-    }
-    __syncthreads();
-}
-
-__device__ __forceinline__ float norm_act(float z, int act) {
-    if (act == NORM_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
-    if (act == NORM_ACT_SILU) {
-        float s, q;
-        plc_sigmoid_pair(z, s, q);
-        return z * s;
-    }
-    return z;
-}
-// act'(z); ReLU's is 0 at 0
-__device__ __forceinline__ float norm_act_slope(float z, int act) {
-    if (act == NORM_ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
-    if (act == NORM_ACT_SILU) {
-        float s, q;
-        plc_sigmoid_pair(z, s, q);
-        return __builtin_fmaf(z * s, q, s);
-    }
-    return 1.0f;
-}
-
-__device__ __forceinline__ PlcDrop norm_drop(const NormArgs& a) {
-    PlcDrop d = a.drop;
-    if (d.thr && a.offset_ptr) d.offset = (uint64_t)*a.offset_ptr;
-    return d;
-}
-
-// (elements are counted in [N][HW][C] order whatever the layout, so that one seed gives one mask)
-template <int V>
-__device__ __forceinline__ uint32_t norm_keep(const NormArgs& a, const PlcDrop& d, int n, int p, int u) {
-    return plc_keep_bits<V>(d, ((uint64_t)n * a.HW + p) * a.C + (uint64_t)u * V);
-}
-
-// per-channel constants of a thread's unit: group mean, r, weight, bias
-template <int V>
-struct NormUnit {
-    float mean[V], r[V], w[V], b[V];
-};
-template <int V>
-__device__ __forceinline__ void norm_unit(const NormArgs& a, int c0, int c, const float* st, NormUnit<V>& k) {
-    const int g0 = c0 / a.cg;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int g = (c + i) / a.cg - g0;
-        k.mean[i] = st[2 * g];
-        k.r[i] = st[2 * g + 1];
-        k.w[i] = a.w ? a.w[c + i] : 1.0f;
-        k.b[i] = a.b ? a.b[c + i] : 0.0f;
-    }
-}
-
-// ---- forward, second pass ---------------------------------------------------------------------------------------
-template <class T, int V>
-__global__ __launch_bounds__(256) void plc_norm_fwd_kernel(NormArgs a) {
-    extern __shared__ __align__(16) float lds[];
-    const NormTid t = norm_tid(a);
-    const NormBlock blk = norm_block(a, blockIdx.x, a.chunks);
-    const int n = blk.n, u0 = blk.tile * a.ut;
-    const int nu = a.U - u0 < a.ut ? a.U - u0 : a.ut;
-    norm_group_stats(a, n, u0 * V, (u0 + nu) * V, lds, blk.range == 0);
-    const PlcDrop drop = norm_drop(a);
-    if (a.used_offset && blockIdx.x == 0 && threadIdx.x == 0) *a.used_offset = (long long)drop.offset;
-    if (!t.on || t.u >= nu) return;
-    NormUnit<V> k;
-    norm_unit<V>(a, u0 * V, (u0 + t.u) * V, lds, k);
-    const long long at = n * a.img + (long long)(u0 + t.u) * a.us;
-    const T* x = (const T*)a.x + at;
-    T* y = (T*)a.y + at;
-    const int p0 = blk.range * a.px_chunk, p1 = p0 + a.px_chunk < a.HW ? p0 + a.px_chunk : a.HW;
-    for (int p = p0 + t.r; p < p1; p += NORM_P * t.rows) {
-        PlcVec<T, V> raw[NORM_P];
-#pragma unroll
-        for (int j = 0; j < NORM_P; ++j)
-            if (p + j * t.rows < p1) raw[j] = plc_load<T, V>(x + (long long)(p + j * t.rows) * a.ps);
-#pragma unroll
-        for (int j = 0; j < NORM_P; ++j) {
-            const int pj = p + j * t.rows;
-            if (pj >= p1) break;
-            const uint32_t keep = drop.thr ? norm_keep<V>(a, drop, n, pj, u0 + t.u) : 0;
-            float o[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float z = __builtin_fmaf(((float)raw[j].e[i] - k.mean[i]) * k.r[i], k.w[i], k.b[i]);
-                o[i] = norm_act(z, a.act);
-                if (drop.thr) o[i] = (keep >> i) & 1 ? o[i] * drop.scale : 0.0f;
-            }
-            plc_store<T, V>(y + (long long)pj * a.ps, plc_from_float<T, V>(o));
-        }
-    }
-}
-
-// ---- backward, first pass: per channel of a pixel range, sum dz and sum dz xh -----------------------------------
-template <class T, int V>
-__device__ __forceinline__ void norm_dz(const NormArgs& a, const NormUnit<V>& k, const PlcDrop& drop, int n, int p, int u,
-                                        const PlcVec<T, V>& xr, const PlcVec<T, V>& gr, float (&xh)[V], float (&dz)[V]) {
-    const uint32_t keep = drop.thr ? norm_keep<V>(a, drop, n, p, u) : 0;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        xh[i] = ((float)xr.e[i] - k.mean[i]) * k.r[i];
-        const float z = __builtin_fmaf(xh[i], k.w[i], k.b[i]);
-        float g = (float)gr.e[i];
-        if (drop.thr) g = (keep >> i) & 1 ? g * drop.scale : 0.0f;
-        dz[i] = a.act == NORM_ACT_NONE ? g : g * norm_act_slope(z, a.act);
-    }
-}
-
-__device__ __forceinline__ void norm_load_stats(const NormArgs& a, int n, int c0, int c1, float* st) {
-    const int g0 = c0 / a.cg, g1 = (c1 - 1) / a.cg;
-    for (int i = threadIdx.x; i < 2 * (g1 - g0 + 1); i += blockDim.x) st[i] = a.stats[((long long)n * a.G + g0) * 2 + i];
-    __syncthreads();
-}
-
-template <class T, int V>
-__global__ __launch_bounds__(256) void plc_norm_bwd_sums_kernel(NormArgs a) {
-    extern __shared__ __align__(16) float lds[];
-    const NormTid t = norm_tid(a);
-    const NormBlock blk = norm_block(a, blockIdx.x, a.splits);
-    const int n = blk.n, u0 = blk.tile * a.ut;
-    const int nu = a.U - u0 < a.ut ? a.U - u0 : a.ut, nch = a.ut * V;
-    norm_load_stats(a, n, u0 * V, (u0 + nu) * V, lds);
-    const PlcDrop drop = norm_drop(a);
-    float v[2][V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[0][i] = v[1][i] = 0.0f;
-    const int p0 = blk.range * a.px_split, p1 = p0 + a.px_split < a.HW ? p0 + a.px_split : a.HW;
-    if (t.on && t.u < nu) {
-        NormUnit<V> k;
-        norm_unit<V>(a, u0 * V, (u0 + t.u) * V, lds, k);
-        const long long at = n * a.img + (long long)(u0 + t.u) * a.us;
-        const T *x = (const T*)a.x + at, *dy = (const T*)a.dy + at;
-        for (int p = p0 + t.r; p < p1; p += NORM_P * t.rows) {
-            PlcVec<T, V> xr[NORM_P], gr[NORM_P];
+        if (p < p1) {
+            PlcVec<T, V> raw[NORM_P];
 #pragma unroll
             for (int j = 0; j < NORM_P; ++j)
-                if (p + j * t.rows < p1) {
-                    xr[j] = plc_load<T, V>(x + (long long)(p + j * t.rows) * a.ps);
-                    gr[j] = plc_load<T, V>(dy + (long long)(p + j * t.rows) * a.ps);
-                }
-#pragma unroll
-            for (int j = 0; j < NORM_P; ++j) {
-                if (p + j * t.rows >= p1) break;
-                float xh[V], dz[V];
-                norm_dz<T, V>(a, k, drop, n, p + j * t.rows, u0 + t.u, xr[j], gr[j], xh, dz);
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    v[0][i] += dz[i];
-                    v[1][i] = __builtin_fmaf(dz[i], xh[i], v[1][i]);
-                }
-            }
+                if (p + j * t.rows < p1) raw[j] = plc_load<T, V>(x + (long long)(p + j * t.rows) * a.ps);
+            merge((p1 - p + t.rows - 1) / t.rows, raw, false);
         }
     }
-    __syncthreads();          // (the statistics in LDS make room for the sums)
-    float* sums = lds;
-    norm_sum_rows<V, 2>(t, a.ut, v, lds + 2 * nch, sums);
-    float* part = a.part + (((long long)n * a.splits + blk.range) * a.C + (long long)u0 * V) * 2;
-    for (int i = threadIdx.x; i < nu * V; i += blockDim.x) {
-        part[2 * i] = sums[i];
-        part[2 * i + 1] = sums[nch + i];
+    // The rows of the workgroup, around the mean of the first row (the pivot is one of the means that are merged, so its
+    // own difference counts in the result and the subtraction loses at most a factor of the number of rows).
+    const int nch = blk.nu * V;
+    float* pivot = lds;
+    float* sums = lds + nch;
+    float* scratch = sums + 2 * nch;
+    if (t.on && t.r == 0)
+#pragma unroll
+        for (int i = 0; i < V; ++i) pivot[t.u * V + i] = mean[i];
+    __syncthreads();
+    float v[2][V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const float d = t.on && count > 0.0f ? mean[i] - pivot[t.u * V + i] : 0.0f;
+        v[0][i] = count * d;
+        v[1][i] = __builtin_fmaf(count * d, d, m2[i]);
+    }
+    norm_sum_rows<V, 2>(t, blk.nu, v, scratch, sums);
+    // channels -> groups, one wave per group
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6, entries = a.splits * a.parts;
+    const int width = a.parts == 1 ? a.cg : nch;
+    const float px = (float)(p1 - p0), inv_px = 1.0f / px, inv_w = 1.0f / (float)width;
+    for (int g = wave; g < blk.ng; g += waves) {
+        float s = 0.0f;
+        for (int c = lane; c < width; c += 64) s += pivot[g * a.cg + c] + sums[g * a.cg + c] * inv_px;
+        const float m = norm_wave_sum(s) * inv_w;
+        float q = 0.0f;
+        for (int c = lane; c < width; c += 64) {
+            const float d0 = sums[g * a.cg + c] * inv_px, d = pivot[g * a.cg + c] + d0 - m;
+            q += sums[nch + g * a.cg + c] + px * (d * d - d0 * d0);
+        }
+        q = norm_wave_sum(q);
+        if (lane == 0) {
+            float* out = a.part_g + (((long long)blk.n * a.G + blk.g0 + g) * entries + blk.range * a.parts + blk.part) * 2;
+            out[0] = m;
+            out[1] = fmaxf(q, 0.0f) + (q != q ? q : 0.0f);
+        }
     }
 }
 
-// ---- backward, second pass: dx; the leading workgroups sum dw and db over samples and ranges -------------------
-// dw, db: 16 channels per workgroup, 16 threads each; the sums over many samples run in 64 bits.
+// pixels times channels of partial sum e of a group
+__device__ __forceinline__ float norm_entry_count(const NormArgs& a, int V, int e) {
+    const int range = e / a.parts, part = e - range * a.parts;
+    const int px = min(a.px_split, a.HW - range * a.px_split);
+    const int ch = a.parts == 1 ? a.cg : min(a.ut, a.gu - part * a.ut) * V;
+    return (float)px * (float)ch;
+}
+
+// ---- split form, forward, second pass ---------------------------------------------------------------------------
+template <class T, int V, int FORM>
+__global__ __launch_bounds__(256) void plc_norm_fwd_kernel(NormArgs a) {
+    extern __shared__ __align__(16) float st[];
+    const NormBlock blk = norm_block<V>(a, blockIdx.x, a.splits);
+    const NormTid t = norm_tid(a, blk);
+    {   // the tile's groups: mean and r from the partial sums, one wave per group
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6, entries = a.splits * a.parts;
+        const float m = (float)a.HW * (float)a.cg;
+        for (int g = wave; g < blk.ng; g += waves) {
+            const float* part = a.part_g + ((long long)blk.n * a.G + blk.g0 + g) * entries * 2;
+            float s = 0.0f, q = 0.0f;
+            for (int e = lane; e < entries; e += 64) s = __builtin_fmaf(norm_entry_count(a, V, e), part[2 * e], s);
+            const float mean = norm_wave_sum(s) / m;
+            for (int e = lane; e < entries; e += 64) {
+                const float d = part[2 * e] - mean;
+                q += __builtin_fmaf(norm_entry_count(a, V, e) * d, d, part[2 * e + 1]);
+            }
+            const float r = 1.0f / sqrtf(norm_wave_sum(q) / m + a.eps);
+            if (lane == 0) {
+                st[2 * g] = mean;
+                st[2 * g + 1] = r;
+                if (blk.range == 0 && blk.part == 0) {
+                    a.stats[((long long)blk.n * a.G + blk.g0 + g) * 2] = mean;
+                    a.stats[((long long)blk.n * a.G + blk.g0 + g) * 2 + 1] = r;
+                }
+            }
+        }
+        __syncthreads();
+    }
+    const PlcDrop drop = norm_drop<FORM>(a);
+    if (a.used_offset && blockIdx.x == 0 && threadIdx.x == 0) *a.used_offset = (long long)drop.offset;
+    if (!t.on) return;
+    NormUnit<V> k;
+    norm_unit<V>(a, blk, t.u, st, k);
+    const int u = blk.u0 + t.u;
+    const long long at = blk.n * a.img + (long long)u * a.us;
+    const T* x = (const T*)a.x + at;
+    T* y = (T*)a.y + at;
+    const int p0 = blk.range * a.px_split, p1 = min(p0 + a.px_split, a.HW);
+    const T* const src[1] = {x};
+    norm_rounds<T, V, NORM_P, 1>(src, a.ps, p0 + t.r, p1, t.rows, [&](int p, const PlcVec<T, V> (&v)[1]) {
+        plc_store<T, V>(y + (long long)p * a.ps, norm_out<T, V, FORM>(a, k, drop, blk.n, p, u, v[0]));
+    });
+}
+
+// ---- backward: sums of a tile ------------------------------------------------------------------------------------
+// v[0] = sum dz, v[1] = sum dz (x - mean) of a thread -> part_c (per channel) and, per group, the sums of w dz and w dz xh:
+// into part_g (split) or as means into LDS (resident)
+template <int V>
+__device__ __forceinline__ void norm_bwd_reduce(const NormArgs& a, const NormBlock& blk, const NormTid& t, const NormUnit<V>& k,
+                                                float (&v)[2][V], float* sums, float* scratch, float* means) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[1][i] *= k.r[i];
+    const int nch = blk.nu * V, c0 = blk.u0 * V;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {         // (one after the other: half the LDS)
+        float one[1][V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) one[0][i] = v[j][i];
+        norm_sum_rows<V, 1>(t, blk.nu, one, scratch, sums + j * nch);
+    }
+    float* out = a.part_c + (((long long)blk.n * a.splits + blk.range) * a.C + c0) * 2;
+    for (int i = threadIdx.x; i < nch; i += blockDim.x) {
+        out[2 * i] = sums[i];
+        out[2 * i + 1] = sums[nch + i];
+    }
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6, entries = a.splits * a.parts;
+    const int width = a.parts == 1 ? a.cg : nch;
+    for (int g = wave; g < blk.ng; g += waves) {
+        float s0 = 0.0f, s1 = 0.0f;
+        for (int c = lane; c < width; c += 64) {
+            const float w = a.w ? a.w[c0 + g * a.cg + c] : 1.0f;
+            s0 = __builtin_fmaf(w, sums[g * a.cg + c], s0);
+            s1 = __builtin_fmaf(w, sums[nch + g * a.cg + c], s1);
+        }
+        s0 = norm_wave_sum(s0);
+        s1 = norm_wave_sum(s1);
+        if (lane == 0) {
+            if (means) {
+                const float m = (float)a.HW * (float)a.cg;
+                means[2 * g] = s0 / m;
+                means[2 * g + 1] = s1 / m;
+            } else {
+                float* pg = a.part_g + (((long long)blk.n * a.G + blk.g0 + g) * entries + blk.range * a.parts + blk.part) * 2;
+                pg[0] = s0;
+                pg[1] = s1;
+            }
+        }
+    }
+}
+
+// dx = rw dz - r c1 - (x - mean) r^2 c2
+template <int V>
+struct NormMeans {
+    float k1[V], k2[V];
+};
+template <int V>
+__device__ __forceinline__ void norm_means(const NormArgs& a, const NormBlock& blk, int u, const float* means, const NormUnit<V>& k, NormMeans<V>& q) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const int g = ((blk.u0 + u) * V + i) / a.cg - blk.g0;
+        q.k1[i] = k.r[i] * means[2 * g];
+        q.k2[i] = k.r[i] * k.r[i] * means[2 * g + 1];
+    }
+}
+template <class T, int V>
+__device__ __forceinline__ PlcVec<T, V> norm_dx(const NormUnit<V>& k, const NormMeans<V>& q, const float (&d)[V], const float (&dz)[V]) {
+    float o[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = __builtin_fmaf(-d[i], q.k2[i], __builtin_fmaf(k.rw[i], dz[i], -q.k1[i]));
+    return plc_from_float<T, V>(o);
+}
+
+// ---- split form, backward, first pass ----------------------------------------------------------------------------
+constexpr int NORM_PB = NORM_P / 2;
+
+template <class T, int V, int FORM>
+__global__ __launch_bounds__(256) void plc_norm_bwd_sums_kernel(NormArgs a) {
+    extern __shared__ __align__(16) float lds[];
+    const NormBlock blk = norm_block<V>(a, blockIdx.x, a.splits);
+    const NormTid t = norm_tid(a, blk);
+    const int nch = blk.nu * V;
+    float* st = lds;
+    norm_load_stats(a, blk, st);
+    const PlcDrop drop = norm_drop<FORM>(a);
+    float v[2][V];
+    NormUnit<V> k;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[0][i] = v[1][i] = k.r[i] = 0.0f;
+    const int p0 = blk.range * a.px_split, p1 = min(p0 + a.px_split, a.HW);
+    if (t.on) {
+        norm_unit<V>(a, blk, t.u, st, k);
+        const int u = blk.u0 + t.u;
+        const long long at = blk.n * a.img + (long long)u * a.us;
+        const T *x = (const T*)a.x + at, *dy = (const T*)a.dy + at;
+        const T* const src[2] = {x, dy};
+        norm_rounds<T, V, NORM_PB, 2>(src, a.ps, p0 + t.r, p1, t.rows, [&](int p, const PlcVec<T, V> (&q)[2]) {
+            float d[V], dz[V];
+            norm_dz<T, V, FORM>(a, k, drop, blk.n, p, u, q[0], q[1], d, dz);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                v[0][i] += dz[i];
+                v[1][i] = __builtin_fmaf(dz[i], d[i], v[1][i]);
+            }
+        });
+    }
+    norm_bwd_reduce<V>(a, blk, t, k, v, lds + 2 * nch, lds + 4 * nch, nullptr);
+}
+
+// ---- backward: dw and db from the per-channel sums of samples and ranges ------------------------------------------
+// 16 channels per workgroup of 256, 16 threads each; the sums over many samples run in 64 bits.
 constexpr int NORM_PARAM_CH = 16;
 
 __device__ __forceinline__ void norm_param_block(const NormArgs& a, int block, double* scratch) {
-    const int c = block * NORM_PARAM_CH + (threadIdx.x & 15), row = threadIdx.x >> 4, rows = blockDim.x >> 4;
+    const int c = block * NORM_PARAM_CH + (threadIdx.x & 15), row = threadIdx.x >> 4;
     double sb = 0.0, sw = 0.0;
-    if (c < a.C)
-        for (long long i = row; i < (long long)a.N * a.splits; i += rows) {
-            sb += (double)a.part[(i * a.C + c) * 2];
-            sw += (double)a.part[(i * a.C + c) * 2 + 1];
+    const long long n = (long long)a.N * a.splits;
+    if (c < a.C) {
+#pragma unroll 8
+        for (long long i = row; i < n; i += 16) {
+            const PlcVec<float, 2> q = plc_load<float, 2>(a.part_c + (i * a.C + c) * 2);
+            sb += (double)q.get(0);
+            sw += (double)q.get(1);
         }
+    }
     scratch[threadIdx.x] = sb;
-    scratch[blockDim.x + threadIdx.x] = sw;
+    scratch[256 + threadIdx.x] = sw;
     __syncthreads();
     if (row == 0 && c < a.C) {
-        for (int i = 1; i < rows; ++i) {
+        for (int i = 1; i < 16; ++i) {
             sb += scratch[i * 16 + threadIdx.x];
-            sw += scratch[blockDim.x + i * 16 + threadIdx.x];
+            sw += scratch[256 + i * 16 + threadIdx.x];
         }
         if (a.db) a.db[c] = (float)sb;
         if (a.dw) a.dw[c] = (float)sw;
     }
 }
+template <class T>        // (T only tells the translation units' copies apart)
+__global__ __launch_bounds__(256) void plc_norm_params_kernel(NormArgs a) {
+    __shared__ double scratch[512];
+    norm_param_block(a, blockIdx.x, scratch);
+}
 
-template <class T, int V>
+// ---- split form, backward, second pass: dx; the leading workgroups sum dw and db -----------------------------------
+template <class T, int V, int FORM>
 __global__ __launch_bounds__(256) void plc_norm_bwd_kernel(NormArgs a) {
     extern __shared__ __align__(16) float lds[];
     if ((int)blockIdx.x < a.param_blocks) {
         norm_param_block(a, blockIdx.x, (double*)lds);
         return;
     }
-    const NormTid t = norm_tid(a);
-    const NormBlock blk = norm_block(a, blockIdx.x - a.param_blocks, a.chunks);
-    const int n = blk.n, u0 = blk.tile * a.ut;
-    const int nu = a.U - u0 < a.ut ? a.U - u0 : a.ut;
-    // means over the group of w dz and w dz xh: one wave per group
-    const int g0 = u0 * V / a.cg, g1 = ((u0 + nu) * V - 1) / a.cg;
+    const NormBlock blk = norm_block<V>(a, blockIdx.x - a.param_blocks, a.splits);
+    const NormTid t = norm_tid(a, blk);
     float* st = lds;
-    float* means = lds + 2 * (g1 - g0 + 1);
+    float* means = lds + 2 * blk.ng;
     {
-        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
-        const long long items = (long long)a.splits * a.cg;
-        for (int g = g0 + wave; g <= g1; g += waves) {
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6, entries = a.splits * a.parts;
+        const float m = (float)a.HW * (float)a.cg;
+        for (int g = wave; g < blk.ng; g += waves) {
+            const float* part = a.part_g + ((long long)blk.n * a.G + blk.g0 + g) * entries * 2;
             float s0 = 0.0f, s1 = 0.0f;
-            for (long long i = lane; i < items; i += 64) {
-                const long long sp = i / a.cg;
-                const int c = g * a.cg + (int)(i - sp * a.cg);
-                const float* part = a.part + (((long long)n * a.splits + sp) * a.C + c) * 2;
-                const float w = a.w ? a.w[c] : 1.0f;
-                s0 = __builtin_fmaf(w, part[0], s0);
-                s1 = __builtin_fmaf(w, part[1], s1);
+            for (int e = lane; e < entries; e += 64) {
+                s0 += part[2 * e];
+                s1 += part[2 * e + 1];
             }
             s0 = norm_wave_sum(s0);
             s1 = norm_wave_sum(s1);
-            const float m = (float)a.HW * (float)a.cg;
             if (lane == 0) {
-                means[2 * (g - g0)] = s0 / m;
-                means[2 * (g - g0) + 1] = s1 / m;
+                means[2 * g] = s0 / m;
+                means[2 * g + 1] = s1 / m;
             }
         }
     }
-    norm_load_stats(a, n, u0 * V, (u0 + nu) * V, st);       // (ends with a barrier)
-    if (!t.on || t.u >= nu) return;
-    const PlcDrop drop = norm_drop(a);
+    norm_load_stats(a, blk, st);       // (ends with a barrier)
+    if (!t.on) return;
+    const PlcDrop drop = norm_drop<FORM>(a);
     NormUnit<V> k;
-    norm_unit<V>(a, u0 * V, (u0 + t.u) * V, st, k);
-    float c1[V], c2[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const int g = ((u0 + t.u) * V + i) / a.cg - g0;
-        c1[i] = means[2 * g];
-        c2[i] = means[2 * g + 1];
-    }
-    const long long at = n * a.img + (long long)(u0 + t.u) * a.us;
+    NormMeans<V> q;
+    norm_unit<V>(a, blk, t.u, st, k);
+    norm_means<V>(a, blk, t.u, means, k, q);
+    const int u = blk.u0 + t.u;
+    const long long at = blk.n * a.img + (long long)u * a.us;
     const T *x = (const T*)a.x + at, *dy = (const T*)a.dy + at;
     T* dx = (T*)a.dx + at;
-    const int p0 = blk.range * a.px_chunk, p1 = p0 + a.px_chunk < a.HW ? p0 + a.px_chunk : a.HW;
-    for (int p = p0 + t.r; p < p1; p += NORM_P * t.rows) {
-        PlcVec<T, V> xr[NORM_P], gr[NORM_P];
+    const int p0 = blk.range * a.px_split, p1 = min(p0 + a.px_split, a.HW);
+    const T* const src[2] = {x, dy};
+    norm_rounds<T, V, NORM_PB, 2>(src, a.ps, p0 + t.r, p1, t.rows, [&](int p, const PlcVec<T, V> (&v)[2]) {
+        float d[V], dz[V];
+        norm_dz<T, V, FORM>(a, k, drop, blk.n, p, u, v[0], v[1], d, dz);
+        plc_store<T, V>(dx + (long long)p * a.ps, norm_dx<T, V>(k, q, d, dz));
+    });
+}
+
+// ---- resident form -----------------------------------------------------------------------------------------------
+// One workgroup per (sample, tile of whole groups); a thread keeps KU units.  Neighbouring tiles share cache lines, so they
+// are given to workgroups of one XCD (workgroups go round the XCDs one by one).
+__device__ __forceinline__ unsigned norm_xcd_order(unsigned i, unsigned n) {
+    const unsigned per = n / 8, rest = n % 8, x = i % 8;
+    return x * per + min(x, rest) + i / 8;
+}
+
+template <class T, int V, int FORM, int KU>
+__global__ __launch_bounds__(512) void plc_norm_fwd_resident_kernel(NormArgs a) {
+    extern __shared__ __align__(16) float lds[];
+    const NormBlock blk = norm_block<V>(a, norm_xcd_order(blockIdx.x, gridDim.x), 1);
+    const NormTid t = norm_tid(a, blk);
+    const int nch = blk.nu * V, u = blk.u0 + t.u;
+    const long long at = blk.n * a.img + (long long)u * a.us;
+    const T* x = (const T*)a.x + at;
+    float* st = lds;
+    float* sums = lds + 2 * blk.ng;
+    float* scratch = sums + nch;
+    const PlcDrop drop = norm_drop<FORM>(a);
+    if (a.used_offset && blockIdx.x == 0 && threadIdx.x == 0) *a.used_offset = (long long)drop.offset;
+    PlcVec<T, V> raw[KU];
 #pragma unroll
-        for (int j = 0; j < NORM_P; ++j)
-            if (p + j * t.rows < p1) {
-                xr[j] = plc_load<T, V>(x + (long long)(p + j * t.rows) * a.ps);
-                gr[j] = plc_load<T, V>(dy + (long long)(p + j * t.rows) * a.ps);
+    for (int j = 0; j < KU; ++j)
+        if (t.on && t.r + j * t.rows < a.HW) raw[j] = plc_load<T, V>(x + (long long)(t.r + j * t.rows) * a.ps);
+    float v[1][V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        v[0][i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < KU; ++j)
+            if (t.on && t.r + j * t.rows < a.HW) v[0][i] += raw[j].get(i);
+    }
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+    const float inv = 1.0f / ((float)a.HW * (float)a.cg);
+    norm_sum_rows<V, 1>(t, blk.nu, v, scratch, sums);
+    for (int g = wave; g < blk.ng; g += waves) {
+        float s = 0.0f;
+        for (int c = lane; c < a.cg; c += 64) s += sums[g * a.cg + c];
+        s = norm_wave_sum(s);
+        if (lane == 0) st[2 * g] = s * inv;
+    }
+    __syncthreads();
+    float mean[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        mean[i] = t.on ? st[2 * ((u * V + i) / a.cg - blk.g0)] : 0.0f;
+        v[0][i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < KU; ++j)
+            if (t.on && t.r + j * t.rows < a.HW) {
+                const float d = raw[j].get(i) - mean[i];
+                v[0][i] = __builtin_fmaf(d, d, v[0][i]);
             }
+    }
+    norm_sum_rows<V, 1>(t, blk.nu, v, scratch, sums);
+    for (int g = wave; g < blk.ng; g += waves) {
+        float s = 0.0f;
+        for (int c = lane; c < a.cg; c += 64) s += sums[g * a.cg + c];
+        s = norm_wave_sum(s);
+        if (lane == 0) {
+            const float r = 1.0f / sqrtf(s * inv + a.eps);
+            st[2 * g + 1] = r;
+            a.stats[((long long)blk.n * a.G + blk.g0 + g) * 2] = st[2 * g];
+            a.stats[((long long)blk.n * a.G + blk.g0 + g) * 2 + 1] = r;
+        }
+    }
+    __syncthreads();
+    if (!t.on) return;
+    NormUnit<V> k;
+    norm_unit<V>(a, blk, t.u, st, k);
+    T* y = (T*)a.y + at;
 #pragma unroll
-        for (int j = 0; j < NORM_P; ++j) {
-            if (p + j * t.rows >= p1) break;
-            float xh[V], dz[V], o[V];
-            norm_dz<T, V>(a, k, drop, n, p + j * t.rows, u0 + t.u, xr[j], gr[j], xh, dz);
+    for (int j = 0; j < KU; ++j) {
+        const int p = t.r + j * t.rows;
+        if (p < a.HW) plc_store<T, V>(y + (long long)p * a.ps, norm_out<T, V, FORM>(a, k, drop, blk.n, p, u, raw[j]));
+    }
+}
+
+template <class T, int V, int FORM, int KU>
+__global__ __launch_bounds__(512) void plc_norm_bwd_resident_kernel(NormArgs a) {
+    extern __shared__ __align__(16) float lds[];
+    const NormBlock blk = norm_block<V>(a, norm_xcd_order(blockIdx.x, gridDim.x), 1);
+    const NormTid t = norm_tid(a, blk);
+    const int nch = blk.nu * V, u = blk.u0 + t.u;
+    const long long at = blk.n * a.img + (long long)u * a.us;
+    const T *x = (const T*)a.x + at, *dy = (const T*)a.dy + at;
+    float* st = lds;
+    float* means = st + 2 * blk.ng;
+    float* sums = means + 2 * blk.ng;
+    float* scratch = sums + 2 * nch;
+    PlcVec<T, V> xr[KU], gr[KU];
 #pragma unroll
-            for (int i = 0; i < V; ++i) o[i] = k.r[i] * (__builtin_fmaf(k.w[i], dz[i], -c1[i]) - xh[i] * c2[i]);
-            plc_store<T, V>(dx + (long long)(p + j * t.rows) * a.ps, plc_from_float<T, V>(o));
+    for (int j = 0; j < KU; ++j)
+        if (t.on && t.r + j * t.rows < a.HW) {
+            xr[j] = plc_load<T, V>(x + (long long)(t.r + j * t.rows) * a.ps);
+            gr[j] = plc_load<T, V>(dy + (long long)(t.r + j * t.rows) * a.ps);
+        }
+    norm_load_stats(a, blk, st);
+    const PlcDrop drop = norm_drop<FORM>(a);
+    float v[2][V];
+    NormUnit<V> k;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[0][i] = v[1][i] = k.r[i] = 0.0f;
+    if (t.on) {
+        norm_unit<V>(a, blk, t.u, st, k);
+#pragma unroll
+        for (int j = 0; j < KU; ++j) {
+            const int p = t.r + j * t.rows;
+            if (p < a.HW) {
+                float d[V], dz[V];
+                norm_dz<T, V, FORM>(a, k, drop, blk.n, p, u, xr[j], gr[j], d, dz);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    v[0][i] += dz[i];
+                    v[1][i] = __builtin_fmaf(dz[i], d[i], v[1][i]);
+                }
+            }
+        }
+    }
+    norm_bwd_reduce<V>(a, blk, t, k, v, sums, scratch, means);
+    __syncthreads();
+    if (!t.on) return;
+    NormMeans<V> q;
+    norm_means<V>(a, blk, t.u, means, k, q);
+    T* dx = (T*)a.dx + at;
+#pragma unroll
+    for (int j = 0; j < KU; ++j) {
+        const int p = t.r + j * t.rows;
+        if (p < a.HW) {
+            float d[V], dz[V];
+            norm_dz<T, V, FORM>(a, k, drop, blk.n, p, u, xr[j], gr[j], d, dz);
+            plc_store<T, V>(dx + (long long)p * a.ps, norm_dx<T, V>(k, q, d, dz));
         }
     }
 }

@@ -8,7 +8,8 @@
 
 // Steps a lane holds in registers at a time: their loads are all requested before the first is used, and the
 // backward pass rebuilds the states of one such block from the state in front of it.
-constexpr int SCAN_K = 16;
+constexpr int SCAN_K = 8;
+constexpr int SCAN_WAVES = 8;         // split form: segments (one per wave) of a workgroup
 
 struct ScanArgs {
     int B, T;
@@ -21,16 +22,28 @@ struct ScanArgs {
     void *y, *dx, *df;              // [B][T][D]
     float *h_last, *dh0;            // [B][D] or null
     float* states;                  // [B][ceil(T / SCAN_K) - 1][D]: the state in front of block 1, 2, ...; or null
+    int seg, nseg;                  // split form: steps of a segment (a multiple of SCAN_K) and their number
+    float* agg;                     // split form: [nseg][2][B * D], what a segment does to the state: h -> A h + S
 };
 
-// One step.  The coupled form is a mean of h and x with weights s and q = 1 - s: it starts from the one with the larger
-// weight and moves by the smaller weight times the difference, which is exact at h = x and at s = 0 and 1, and loses
-// nothing of a gate near 1 (q is not formed by subtraction).
-__device__ __forceinline__ float scan_step(float h, float x, float s, float q, bool coupled) {
-    if (!coupled) return __builtin_fmaf(s, h, x);
-    const bool open = q < s;
-    const float d = x - h;
-    return __builtin_fmaf(open ? q : -s, d, open ? h : x);
+// The gate as one number, w = -(1 - s) for s > 1/2 and s otherwise: the smaller of the two weights with the sign telling
+// which it is.  Both weights follow from it to half a step (1 - |w| >= 1/2), so one register keeps what two would.
+// e = exp(-|f|) in (0, 1], |w| = e / (1 + e).  For fp32 tensors the product |f| log2(e) is taken in two parts; for 16-bit
+// ones its rounding (|f| 2^-24 relative in e, hence at most 0.4 2^-24 in |w|) is far below their own.
+template <class T>
+__device__ __forceinline__ float scan_gate(float f) {
+    const float e = sizeof(T) == 4 ? plc_exp_neg(-__builtin_fabsf(f)) : __builtin_amdgcn_exp2f(-1.44269504088896341f * __builtin_fabsf(f));
+    return __builtin_copysignf(e * __builtin_amdgcn_rcpf(1.0f + e), -f);
+}
+__device__ __forceinline__ bool scan_open(float w) { return __builtin_bit_cast(int, w) < 0; }     // (-0.0: s = 1)
+__device__ __forceinline__ float scan_s(float w) { return scan_open(w) ? 1.0f + w : w; }
+
+// One step.  The coupled form is a mean of h and x: it starts from the one with the larger weight and moves by the smaller
+// weight times the difference, which is exact at h = x and at s = 0 and 1, and loses nothing of a gate near 1.
+template <bool COUPLED>
+__device__ __forceinline__ float scan_step(float h, float x, float w) {
+    if (!COUPLED) return __builtin_fmaf(scan_s(w), h, x);
+    return __builtin_fmaf(-w, x - h, scan_open(w) ? h : x);
 }
 
 struct ScanLane {
@@ -38,8 +51,8 @@ struct ScanLane {
     int n;            // steps of this sample
 };
 template <int V>
-__device__ __forceinline__ bool scan_lane(const ScanArgs& a, ScanLane& l) {
-    const long long per = a.D / V, i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+__device__ __forceinline__ bool scan_lane(const ScanArgs& a, long long i, ScanLane& l) {
+    const long long per = a.D / V;
     if (i >= per * a.B) return false;
     l.b = i / per;
     l.d = (i - l.b * per) * V;
@@ -52,126 +65,269 @@ __device__ __forceinline__ bool scan_lane(const ScanArgs& a, ScanLane& l) {
 }
 
 template <int V>
-__device__ __forceinline__ void scan_load_state(const float* p, long long b, long long D, long long d, float (&h)[V]) {
+__device__ __forceinline__ void scan_load_state(const float* p, long long at, float (&h)[V]) {
     if (p) {
-        plc_to_float<float, V>(plc_load<float, V>(p + b * D + d), h);
+        plc_to_float<float, V>(plc_load<float, V>(p + at), h);
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) h[i] = 0.0f;
     }
 }
 
-// forward, one lane from the first step to the last
-template <class T, int V>
+// rows t0 .. t0 + SCAN_K - 1 of one tensor; rows from n on are not read (FULL: there are none)
+template <class T, int V, bool FULL>
+__device__ __forceinline__ void scan_rows(const void* base, long long sb, long long st, const ScanLane& l, int t0, PlcVec<T, V> (&r)[SCAN_K]) {
+    const T* p = (const T*)base + l.b * sb + l.d + t0 * st;
+#pragma unroll
+    for (int j = 0; j < SCAN_K; ++j)
+        if (FULL || t0 + j < l.n) r[j] = plc_load<T, V>(p + j * st);
+}
+
+// ---- forward ----------------------------------------------------------------------------------------------------
+// one block of steps from state h; rows between the sample's length and T get 0
+template <class T, int V, bool COUPLED, bool FULL>
+__device__ __forceinline__ void scan_fwd_block(const ScanArgs& a, const ScanLane& l, int t0, float (&h)[V]) {
+    PlcVec<T, V> xr[SCAN_K], fr[SCAN_K];
+    scan_rows<T, V, FULL>(a.f, a.f_sb, a.f_st, l, t0, fr);
+    scan_rows<T, V, FULL>(a.x, a.x_sb, a.x_st, l, t0, xr);
+    T* y = (T*)a.y + (l.b * a.T + t0) * a.D + l.d;
+#pragma unroll
+    for (int j = 0; j < SCAN_K; ++j) {
+        if (!FULL && t0 + j >= a.T) break;
+        float o[V];
+        const bool on = FULL || t0 + j < l.n;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if (on) h[i] = scan_step<COUPLED>(h[i], xr[j].get(i), scan_gate<T>(fr[j].get(i)));
+            o[i] = on ? h[i] : 0.0f;
+        }
+        plc_store<T, V>(y + j * a.D, plc_from_float<T, V>(o));
+    }
+}
+template <class T, int V, bool COUPLED>
+__device__ __forceinline__ void scan_fwd_range(const ScanArgs& a, const ScanLane& l, int t0, int t1, float (&h)[V]) {
+    const int blocks = (a.T + SCAN_K - 1) / SCAN_K;
+    for (int t = t0; t < t1; t += SCAN_K) {
+        const int k = t / SCAN_K;
+        if (k > 0 && a.states) plc_store<float, V>(a.states + (l.b * (blocks - 1) + k - 1) * a.D + l.d, plc_from_float<float, V>(h));
+        if (__all(t + SCAN_K <= l.n)) scan_fwd_block<T, V, COUPLED, true>(a, l, t, h);
+        else scan_fwd_block<T, V, COUPLED, false>(a, l, t, h);
+    }
+}
+
+// one lane from the first step to the last
+template <class T, int V, bool COUPLED>
 __global__ __launch_bounds__(256) void plc_scan_fwd_kernel(ScanArgs a) {
     ScanLane l;
-    if (!scan_lane<V>(a, l)) return;
-    const T* x = (const T*)a.x + l.b * a.x_sb + l.d;
-    const T* f = (const T*)a.f + l.b * a.f_sb + l.d;
-    T* y = (T*)a.y + l.b * a.T * a.D + l.d;
+    if (!scan_lane<V>(a, (long long)blockIdx.x * blockDim.x + threadIdx.x, l)) return;
     float h[V];
-    scan_load_state<V>(a.h0, l.b, a.D, l.d, h);
-    const int blocks = (a.T + SCAN_K - 1) / SCAN_K;
-    for (int k = 0; k < blocks; ++k) {
-        const int t0 = k * SCAN_K;
-        if (k > 0 && a.states)
-            plc_store<float, V>(a.states + (l.b * (blocks - 1) + k - 1) * a.D + l.d, plc_from_float<float, V>(h));
-        PlcVec<T, V> xr[SCAN_K], fr[SCAN_K];
-#pragma unroll
-        for (int j = 0; j < SCAN_K; ++j)
-            if (t0 + j < l.n) {
-                xr[j] = plc_load<T, V>(x + (t0 + j) * a.x_st);
-                fr[j] = plc_load<T, V>(f + (t0 + j) * a.f_st);
-            }
-#pragma unroll
-        for (int j = 0; j < SCAN_K; ++j) {
-            if (t0 + j >= a.T) break;
-            float o[V];
-            if (t0 + j < l.n) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    float s, q;
-                    plc_sigmoid_pair((float)fr[j].e[i], s, q);
-                    h[i] = scan_step(h[i], (float)xr[j].e[i], s, q, a.coupled);
-                    o[i] = h[i];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) o[i] = 0.0f;
-            }
-            plc_store<T, V>(y + (t0 + j) * a.D, plc_from_float<T, V>(o));
-        }
-    }
+    scan_load_state<V>(a.h0, l.b * a.D + l.d, h);
+    scan_fwd_range<T, V, COUPLED>(a, l, 0, a.T, h);
     if (a.h_last) plc_store<float, V>(a.h_last + l.b * a.D + l.d, plc_from_float<float, V>(h));
 }
 
-// backward of one block of steps: rebuilds h in fp32 from the state in front of it, then walks it from the end.
+// ---- backward ---------------------------------------------------------------------------------------------------
+// One block of steps: rebuilds the states in fp32 from the one in front of it, then walks it from the end.
 // p: what the steps behind the block pass to their previous state (s_{t+1} g_{t+1}); on return, what this block
-// passes on.
-template <class T, int V>
+// passes on.  Between the two walks a step is two numbers per channel: its gate, and the factor of df (h_{t-1} - x_t or
+// h_{t-1}); x and f are not kept.
+template <class T, int V, bool COUPLED, bool FULL>
 __device__ __forceinline__ void scan_bwd_block(const ScanArgs& a, const ScanLane& l, int t0, float (&h)[V], float (&p)[V]) {
-    const T* x = (const T*)a.x + l.b * a.x_sb + l.d;
-    const T* f = (const T*)a.f + l.b * a.f_sb + l.d;
-    const T* dy = (const T*)a.dy + l.b * a.dy_sb + l.d;
-    T* dx = (T*)a.dx + l.b * a.T * a.D + l.d;
-    T* df = (T*)a.df + l.b * a.T * a.D + l.d;
-    PlcVec<T, V> xr[SCAN_K], fr[SCAN_K], gr[SCAN_K];
+    PlcVec<T, V> gr[SCAN_K];
+    float w[SCAN_K][V], m[SCAN_K][V];
+    {
+        PlcVec<T, V> xr[SCAN_K], fr[SCAN_K];
+        scan_rows<T, V, FULL>(a.f, a.f_sb, a.f_st, l, t0, fr);
+        scan_rows<T, V, FULL>(a.x, a.x_sb, a.x_st, l, t0, xr);
+        scan_rows<T, V, FULL>(a.dy, a.dy_sb, a.dy_st, l, t0, gr);
 #pragma unroll
-    for (int j = 0; j < SCAN_K; ++j)
-        if (t0 + j < l.n) {
-            xr[j] = plc_load<T, V>(x + (t0 + j) * a.x_st);
-            fr[j] = plc_load<T, V>(f + (t0 + j) * a.f_st);
-            gr[j] = plc_load<T, V>(dy + (t0 + j) * a.dy_st);
+        for (int j = 0; j < SCAN_K; ++j) {
+            const bool on = FULL || t0 + j < l.n;
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (on) {
+                    const float x = xr[j].get(i);
+                    w[j][i] = scan_gate<T>(fr[j].get(i));
+                    m[j][i] = COUPLED ? h[i] - x : h[i];
+                    h[i] = scan_step<COUPLED>(h[i], x, w[j][i]);
+                }
         }
-    float before[SCAN_K][V];        // the state in front of each step
-#pragma unroll
-    for (int j = 0; j < SCAN_K; ++j)
-        if (t0 + j < l.n) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                float s, q;
-                plc_sigmoid_pair((float)fr[j].e[i], s, q);
-                before[j][i] = h[i];
-                h[i] = scan_step(h[i], (float)xr[j].e[i], s, q, a.coupled);
-            }
-        }
+    }
+    T* dx = (T*)a.dx + (l.b * a.T + t0) * a.D + l.d;
+    T* df = (T*)a.df + (l.b * a.T + t0) * a.D + l.d;
 #pragma unroll
     for (int j = SCAN_K - 1; j >= 0; --j) {
-        if (t0 + j >= a.T) continue;
+        if (!FULL && t0 + j >= a.T) continue;
+        const bool on = FULL || t0 + j < l.n;
         float ox[V], of[V];
-        if (t0 + j < l.n) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                float s, q;
-                plc_sigmoid_pair((float)fr[j].e[i], s, q);
-                const float g = (float)gr[j].e[i] + p[i];
-                const float m = a.coupled ? before[j][i] - (float)xr[j].e[i] : before[j][i];
-                ox[i] = a.coupled ? q * g : g;
-                of[i] = g * m * (s * q);
+        for (int i = 0; i < V; ++i) {
+            if (on) {
+                const float small = __builtin_fabsf(w[j][i]), large = 1.0f - small;
+                const bool open = scan_open(w[j][i]);
+                const float s = open ? large : small, g = gr[j].get(i) + p[i];
+                ox[i] = COUPLED ? (open ? small : large) * g : g;
+                of[i] = g * m[j][i] * (small * large);
                 p[i] = s * g;
+            } else {
+                ox[i] = of[i] = 0.0f;
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) ox[i] = of[i] = 0.0f;
         }
-        plc_store<T, V>(dx + (t0 + j) * a.D, plc_from_float<T, V>(ox));
-        plc_store<T, V>(df + (t0 + j) * a.D, plc_from_float<T, V>(of));
+        plc_store<T, V>(dx + j * a.D, plc_from_float<T, V>(ox));
+        plc_store<T, V>(df + j * a.D, plc_from_float<T, V>(of));
+    }
+}
+template <class T, int V, bool COUPLED>
+__device__ __forceinline__ void scan_bwd_range(const ScanArgs& a, const ScanLane& l, int t0, int t1, float (&p)[V]) {
+    const int blocks = (a.T + SCAN_K - 1) / SCAN_K;
+    for (int k = (t1 - 1) / SCAN_K; k >= t0 / SCAN_K; --k) {
+        float h[V];
+        if (k > 0) scan_load_state<V>(a.states, (l.b * (blocks - 1) + k - 1) * a.D + l.d, h);
+        else scan_load_state<V>(a.h0, l.b * a.D + l.d, h);
+        if (__all((k + 1) * SCAN_K <= l.n)) scan_bwd_block<T, V, COUPLED, true>(a, l, k * SCAN_K, h, p);
+        else scan_bwd_block<T, V, COUPLED, false>(a, l, k * SCAN_K, h, p);
     }
 }
 
-// backward, one lane from the last step to the first
-template <class T, int V>
+// one lane from the last step to the first
+template <class T, int V, bool COUPLED>
 __global__ __launch_bounds__(256) void plc_scan_bwd_kernel(ScanArgs a) {
     ScanLane l;
-    if (!scan_lane<V>(a, l)) return;
+    if (!scan_lane<V>(a, (long long)blockIdx.x * blockDim.x + threadIdx.x, l)) return;
     float p[V];
-    scan_load_state<V>(a.dh_last, l.b, a.D, l.d, p);
-    const int blocks = (a.T + SCAN_K - 1) / SCAN_K;
-    for (int k = blocks - 1; k >= 0; --k) {
-        float h[V];
-        if (k > 0) scan_load_state<V>(a.states + (l.b * (blocks - 1) + k - 1) * a.D, 0, 0, l.d, h);
-        else scan_load_state<V>(a.h0, l.b, a.D, l.d, h);
-        scan_bwd_block<T, V>(a, l, k * SCAN_K, h, p);
-    }
+    scan_load_state<V>(a.dh_last, l.b * a.D + l.d, p);
+    if (a.T > 0) scan_bwd_range<T, V, COUPLED>(a, l, 0, a.T, p);
     if (a.dh0) plc_store<float, V>(a.dh0 + l.b * a.D + l.d, plc_from_float<float, V>(p));
+}
+
+// ---- split form: few channels, many steps -----------------------------------------------------------------------
+// A segment of steps does h -> A h + S to the state (A the product of its gates), and the same to the gradient that runs
+// backwards, p -> A p + S.  The first launch computes A and S of every segment (one wave per segment and 64 lanes), the
+// second folds those in front of (behind) its segment into the state it starts from and walks the segment as above.  x and f
+// (f and dy) are read twice, the second time mostly from the cache; in return every segment runs at once.
+template <class T, int V, bool COUPLED, bool BACKWARD, bool FULL>
+__device__ __forceinline__ void scan_agg_block(const ScanArgs& a, const ScanLane& l, int t0, float (&A)[V], float (&S)[V]) {
+    PlcVec<T, V> fr[SCAN_K], vr[SCAN_K];
+    scan_rows<T, V, FULL>(a.f, a.f_sb, a.f_st, l, t0, fr);
+    if (BACKWARD) scan_rows<T, V, FULL>(a.dy, a.dy_sb, a.dy_st, l, t0, vr);
+    else scan_rows<T, V, FULL>(a.x, a.x_sb, a.x_st, l, t0, vr);
+#pragma unroll
+    for (int jj = 0; jj < SCAN_K; ++jj) {
+        const int j = BACKWARD ? SCAN_K - 1 - jj : jj;
+        if (FULL || t0 + j < l.n) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float w = scan_gate<T>(fr[j].get(i)), v = vr[j].get(i), s = scan_s(w);
+                A[i] *= s;
+                S[i] = BACKWARD ? s * (v + S[i]) : scan_step<COUPLED>(S[i], v, w);
+            }
+        }
+    }
+}
+
+// workgroup: SCAN_WAVES segments of 64 lanes; blockIdx.x = group of segments + number of groups * tile of lanes
+struct ScanSeg {
+    int first, k, wave, lane;       // first segment of the workgroup, this wave's, ...
+    long long i;
+};
+__device__ __forceinline__ ScanSeg scan_seg(const ScanArgs& a) {
+    ScanSeg s;
+    const unsigned groups = (a.nseg + SCAN_WAVES - 1) / SCAN_WAVES, tile = blockIdx.x / groups;
+    s.wave = threadIdx.x >> 6;
+    s.lane = threadIdx.x & 63;
+    s.first = (int)(blockIdx.x - tile * groups) * SCAN_WAVES;
+    s.k = s.first + s.wave;
+    s.i = (long long)tile * 64 + s.lane;
+    return s;
+}
+
+template <class T, int V, bool COUPLED, bool BACKWARD>
+__global__ __launch_bounds__(64 * SCAN_WAVES) void plc_scan_segments_kernel(ScanArgs a) {
+    const ScanSeg s = scan_seg(a);
+    ScanLane l;
+    if (s.k >= a.nseg || !scan_lane<V>(a, s.i, l)) return;
+    float A[V], S[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) A[i] = 1.0f, S[i] = 0.0f;
+    const int t0 = s.k * a.seg, t1 = min(t0 + a.seg, a.T), blocks = (t1 - t0 + SCAN_K - 1) / SCAN_K;
+    for (int q = 0; q < blocks; ++q) {
+        const int t = t0 + (BACKWARD ? blocks - 1 - q : q) * SCAN_K;
+        if (__all(t + SCAN_K <= l.n)) scan_agg_block<T, V, COUPLED, BACKWARD, true>(a, l, t, A, S);
+        else scan_agg_block<T, V, COUPLED, BACKWARD, false>(a, l, t, A, S);
+    }
+    float* agg = a.agg + (long long)s.k * 2 * a.B * a.D + l.b * a.D + l.d;
+    plc_store<float, V>(agg, plc_from_float<float, V>(A));
+    plc_store<float, V>(agg + (long long)a.B * a.D, plc_from_float<float, V>(S));
+}
+
+// (A, S) after segments k0, k0 + step, ... (count of them)
+template <int V>
+__device__ __forceinline__ void scan_fold(const float* agg, long long n, long long stride, int count, float (&A)[V], float (&S)[V]) {
+    constexpr int U = 8;
+    for (int q = 0; q < count; q += U) {
+        PlcVec<float, V> ra[U], rs[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+            if (q + j < count) {
+                ra[j] = plc_load<float, V>(agg + (q + j) * stride);
+                rs[j] = plc_load<float, V>(agg + (q + j) * stride + n);
+            }
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+            if (q + j < count) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    S[i] = __builtin_fmaf(ra[j].get(i), S[i], rs[j].get(i));
+                    A[i] *= ra[j].get(i);
+                }
+            }
+    }
+}
+
+template <class T, int V, bool COUPLED, bool BACKWARD>
+__global__ __launch_bounds__(64 * SCAN_WAVES) void plc_scan_split_kernel(ScanArgs a) {
+    __shared__ float part[2][SCAN_WAVES][64 * V];
+    const ScanSeg s = scan_seg(a);
+    ScanLane l;
+    const bool on = scan_lane<V>(a, s.i, l);
+    const long long n = (long long)a.B * a.D, per = 2 * n;
+    // the segments outside the workgroup that come first (forward: in front of it, backward: behind it), an equal share to
+    // each wave, joined in order through LDS
+    const int last = min(s.first + SCAN_WAVES, a.nseg);               // one behind the workgroup's segments
+    const int before = BACKWARD ? a.nseg - last : s.first;
+    const int share = (before + SCAN_WAVES - 1) / SCAN_WAVES;
+    const int q0 = min(s.wave * share, before), q1 = min(q0 + share, before);
+    float A[V], S[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) A[i] = 1.0f, S[i] = 0.0f;
+    const float* agg = a.agg + l.b * a.D + l.d;
+    if (on && q1 > q0) {
+        if (BACKWARD) scan_fold<V>(agg + (a.nseg - 1 - q0) * per, n, -per, q1 - q0, A, S);
+        else scan_fold<V>(agg + q0 * per, n, per, q1 - q0, A, S);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        part[0][s.wave][s.lane * V + i] = A[i];
+        part[1][s.wave][s.lane * V + i] = S[i];
+    }
+    __syncthreads();
+    if (!on || s.k >= a.nseg) return;
+    float h[V];
+    scan_load_state<V>(BACKWARD ? a.dh_last : a.h0, l.b * a.D + l.d, h);
+    for (int q = 0; q < SCAN_WAVES; ++q)
+#pragma unroll
+        for (int i = 0; i < V; ++i) h[i] = __builtin_fmaf(part[0][q][s.lane * V + i], h[i], part[1][q][s.lane * V + i]);
+    float one[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) one[i] = 1.0f;
+    const int t0 = s.k * a.seg, t1 = min(t0 + a.seg, a.T);
+    if (BACKWARD) {
+        scan_fold<V>(agg + (last - 1) * per, n, -per, last - 1 - s.k, one, h);
+        scan_bwd_range<T, V, COUPLED>(a, l, t0, t1, h);
+        if (s.k == 0 && a.dh0) plc_store<float, V>(a.dh0 + l.b * a.D + l.d, plc_from_float<float, V>(h));
+    } else {
+        scan_fold<V>(agg + s.first * per, n, per, s.wave, one, h);
+        scan_fwd_range<T, V, COUPLED>(a, l, t0, t1, h);
+        if (s.k == a.nseg - 1 && a.h_last) plc_store<float, V>(a.h_last + l.b * a.D + l.d, plc_from_float<float, V>(h));
+    }
 }

@@ -331,7 +331,7 @@ def group_norm_forward(x, groups, weight=None, bias=None, eps=1e-5, act="none", 
     stats = torch.empty((x.shape[0], groups, 2), dtype=torch.float32, device=x.device)
     d = _norm_desc(x, groups, weight, bias, eps, act, p, seed, off, off_t, stats)
     d.y, d.used_offset = y.data_ptr(), _ptr(used_offset)
-    n = L.plc_group_norm_workspace_bytes(C.byref(d))
+    n = L.plc_group_norm_workspace_bytes(C.byref(d), 0)
     ws = workspace(n, x.device)
     d.workspace, d.workspace_bytes = ws.data_ptr(), n
     with _Launch(x.device) as stream:
@@ -356,7 +356,7 @@ def group_norm_backward(x, groups, weight, bias, eps, act, p, seed, offset, stat
     db = torch.empty_like(bias) if bias is not None else None
     d = _norm_desc(x, groups, weight, bias, eps, act, p, seed, off, off_t, stats)
     d.dy, d.dx, d.dweight, d.dbias = dy.data_ptr(), dx.data_ptr(), _ptr(dw), _ptr(db)
-    n = L.plc_group_norm_workspace_bytes(C.byref(d))
+    n = L.plc_group_norm_workspace_bytes(C.byref(d), 1)
     ws = workspace(n, x.device)
     d.workspace, d.workspace_bytes = ws.data_ptr(), n
     with _Launch(x.device) as stream:

@@ -61,7 +61,7 @@ def test_scan_abi_refusals():
     refused(L.plc_gated_scan_fwd(C.byref(scan_desc(B=1 << 30, D=1 << 20)), None), -2, "one launch")
     # nothing to do is no error
     assert L.plc_gated_scan_fwd(C.byref(scan_desc(B=0, x=None, f=None, y=None)), None) == 0
-    assert L.plc_gated_scan_states_bytes(2, 16, 8) == 0 and L.plc_gated_scan_states_bytes(2, 33, 8) == 2 * 2 * 8 * 4
+    assert L.plc_gated_scan_states_bytes(2, 8, 8) == 0 and L.plc_gated_scan_states_bytes(2, 33, 8) == 2 * 4 * 8 * 4
     assert L.plc_gated_scan_states_bytes(0, 33, 8) == 0
 
 
@@ -78,8 +78,8 @@ def test_norm_abi_refusals():
     refused(L.plc_group_norm_bwd(C.byref(norm_desc(dy=None)), None), -1, "null tensor")
     refused(L.plc_group_norm_fwd(C.byref(norm_desc(workspace_bytes=1)), None), -3, "workspace")
     refused(L.plc_group_norm_fwd(C.byref(norm_desc(N=(1 << 31) - 1, workspace_bytes=1 << 50)), None), -2, "one launch")
-    need = L.plc_group_norm_workspace_bytes(C.byref(norm_desc()))
-    assert need > 0 and L.plc_group_norm_workspace_bytes(C.byref(norm_desc(G=5))) == 0
+    need = L.plc_group_norm_workspace_bytes(C.byref(norm_desc()), 0)
+    assert need > 0 and L.plc_group_norm_workspace_bytes(C.byref(norm_desc(G=5)), 1) == 0
     assert L.plc_group_norm_fwd(C.byref(norm_desc(N=0, x=None, y=None)), None) == 0
 
 
