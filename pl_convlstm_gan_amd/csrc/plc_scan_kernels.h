@@ -74,13 +74,14 @@ __device__ __forceinline__ void scan_load_state(const float* p, long long at, fl
     }
 }
 
-// rows t0 .. t0 + SCAN_K - 1 of one tensor; rows from n on are not read (FULL: there are none)
+// Rows t0 .. t0 + SCAN_K - 1 of one tensor.  Not FULL: the block reaches behind some lane's sample.  Its loads are not
+// conditional all the same (they would wait for one another); a row behind the sequence becomes its last one, which is
+// memory of the tensor, and what is loaded there is not used.
 template <class T, int V, bool FULL>
-__device__ __forceinline__ void scan_rows(const void* base, long long sb, long long st, const ScanLane& l, int t0, PlcVec<T, V> (&r)[SCAN_K]) {
-    const T* p = (const T*)base + l.b * sb + l.d + t0 * st;
+__device__ __forceinline__ void scan_rows(const ScanArgs& a, const void* base, long long sb, long long st, const ScanLane& l, int t0, PlcVec<T, V> (&r)[SCAN_K]) {
+    const T* p = (const T*)base + l.b * sb + l.d;
 #pragma unroll
-    for (int j = 0; j < SCAN_K; ++j)
-        if (FULL || t0 + j < l.n) r[j] = plc_load<T, V>(p + j * st);
+    for (int j = 0; j < SCAN_K; ++j) r[j] = plc_load<T, V>(p + (FULL ? t0 + j : min(t0 + j, a.T - 1)) * st);
 }
 
 // ---- forward ----------------------------------------------------------------------------------------------------
@@ -88,8 +89,8 @@ __device__ __forceinline__ void scan_rows(const void* base, long long sb, long l
 template <class T, int V, bool COUPLED, bool FULL>
 __device__ __forceinline__ void scan_fwd_block(const ScanArgs& a, const ScanLane& l, int t0, float (&h)[V]) {
     PlcVec<T, V> xr[SCAN_K], fr[SCAN_K];
-    scan_rows<T, V, FULL>(a.f, a.f_sb, a.f_st, l, t0, fr);
-    scan_rows<T, V, FULL>(a.x, a.x_sb, a.x_st, l, t0, xr);
+    scan_rows<T, V, FULL>(a, a.f, a.f_sb, a.f_st, l, t0, fr);
+    scan_rows<T, V, FULL>(a, a.x, a.x_sb, a.x_st, l, t0, xr);
     T* y = (T*)a.y + (l.b * a.T + t0) * a.D + l.d;
 #pragma unroll
     for (int j = 0; j < SCAN_K; ++j) {
@@ -98,11 +99,23 @@ __device__ __forceinline__ void scan_fwd_block(const ScanArgs& a, const ScanLane
         const bool on = FULL || t0 + j < l.n;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            if (on) h[i] = scan_step<COUPLED>(h[i], xr[j].get(i), scan_gate<T>(fr[j].get(i)));
-            o[i] = on ? h[i] : 0.0f;
+            const float next = scan_step<COUPLED>(h[i], xr[j].get(i), scan_gate<T>(fr[j].get(i)));
+            h[i] = on ? next : h[i];
+            o[i] = on ? next : 0.0f;
         }
         plc_store<T, V>(y + j * a.D, plc_from_float<T, V>(o));
     }
+}
+// a block behind every lane's sample
+template <class T, int V>
+__device__ __forceinline__ void scan_zero_block(const ScanArgs& a, T* y, const ScanLane& l, int t0) {
+    float o[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = 0.0f;
+    y += (l.b * a.T + t0) * a.D + l.d;
+#pragma unroll
+    for (int j = 0; j < SCAN_K; ++j)
+        if (t0 + j < a.T) plc_store<T, V>(y + j * a.D, plc_from_float<T, V>(o));
 }
 template <class T, int V, bool COUPLED>
 __device__ __forceinline__ void scan_fwd_range(const ScanArgs& a, const ScanLane& l, int t0, int t1, float (&h)[V]) {
@@ -111,7 +124,8 @@ __device__ __forceinline__ void scan_fwd_range(const ScanArgs& a, const ScanLane
         const int k = t / SCAN_K;
         if (k > 0 && a.states) plc_store<float, V>(a.states + (l.b * (blocks - 1) + k - 1) * a.D + l.d, plc_from_float<float, V>(h));
         if (__all(t + SCAN_K <= l.n)) scan_fwd_block<T, V, COUPLED, true>(a, l, t, h);
-        else scan_fwd_block<T, V, COUPLED, false>(a, l, t, h);
+        else if (__any(t < l.n)) scan_fwd_block<T, V, COUPLED, false>(a, l, t, h);
+        else scan_zero_block<T, V>(a, (T*)a.y, l, t);
     }
 }
 
@@ -137,20 +151,20 @@ __device__ __forceinline__ void scan_bwd_block(const ScanArgs& a, const ScanLane
     float w[SCAN_K][V], m[SCAN_K][V];
     {
         PlcVec<T, V> xr[SCAN_K], fr[SCAN_K];
-        scan_rows<T, V, FULL>(a.f, a.f_sb, a.f_st, l, t0, fr);
-        scan_rows<T, V, FULL>(a.x, a.x_sb, a.x_st, l, t0, xr);
-        scan_rows<T, V, FULL>(a.dy, a.dy_sb, a.dy_st, l, t0, gr);
+        scan_rows<T, V, FULL>(a, a.f, a.f_sb, a.f_st, l, t0, fr);
+        scan_rows<T, V, FULL>(a, a.x, a.x_sb, a.x_st, l, t0, xr);
+        scan_rows<T, V, FULL>(a, a.dy, a.dy_sb, a.dy_st, l, t0, gr);
 #pragma unroll
         for (int j = 0; j < SCAN_K; ++j) {
             const bool on = FULL || t0 + j < l.n;
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if (on) {
-                    const float x = xr[j].get(i);
-                    w[j][i] = scan_gate<T>(fr[j].get(i));
-                    m[j][i] = COUPLED ? h[i] - x : h[i];
-                    h[i] = scan_step<COUPLED>(h[i], x, w[j][i]);
-                }
+            for (int i = 0; i < V; ++i) {
+                const float x = xr[j].get(i);
+                w[j][i] = scan_gate<T>(fr[j].get(i));
+                m[j][i] = COUPLED ? h[i] - x : h[i];
+                const float next = scan_step<COUPLED>(h[i], x, w[j][i]);
+                h[i] = on ? next : h[i];
+            }
         }
     }
     T* dx = (T*)a.dx + (l.b * a.T + t0) * a.D + l.d;
@@ -162,16 +176,12 @@ __device__ __forceinline__ void scan_bwd_block(const ScanArgs& a, const ScanLane
         float ox[V], of[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            if (on) {
-                const float small = __builtin_fabsf(w[j][i]), large = 1.0f - small;
-                const bool open = scan_open(w[j][i]);
-                const float s = open ? large : small, g = gr[j].get(i) + p[i];
-                ox[i] = COUPLED ? (open ? small : large) * g : g;
-                of[i] = g * m[j][i] * (small * large);
-                p[i] = s * g;
-            } else {
-                ox[i] = of[i] = 0.0f;
-            }
+            const float small = __builtin_fabsf(w[j][i]), large = 1.0f - small;
+            const bool open = scan_open(w[j][i]);
+            const float s = open ? large : small, g = gr[j].get(i) + p[i];
+            ox[i] = on ? (COUPLED ? (open ? small : large) * g : g) : 0.0f;
+            of[i] = on ? g * m[j][i] * (small * large) : 0.0f;
+            p[i] = on ? s * g : p[i];
         }
         plc_store<T, V>(dx + j * a.D, plc_from_float<T, V>(ox));
         plc_store<T, V>(df + j * a.D, plc_from_float<T, V>(of));
@@ -184,6 +194,11 @@ __device__ __forceinline__ void scan_bwd_range(const ScanArgs& a, const ScanLane
         float h[V];
         if (k > 0) scan_load_state<V>(a.states, (l.b * (blocks - 1) + k - 1) * a.D + l.d, h);
         else scan_load_state<V>(a.h0, l.b * a.D + l.d, h);
+        if (!__any(k * SCAN_K < l.n)) {
+            scan_zero_block<T, V>(a, (T*)a.dx, l, k * SCAN_K);
+            scan_zero_block<T, V>(a, (T*)a.df, l, k * SCAN_K);
+            continue;
+        }
         if (__all((k + 1) * SCAN_K <= l.n)) scan_bwd_block<T, V, COUPLED, true>(a, l, k * SCAN_K, h, p);
         else scan_bwd_block<T, V, COUPLED, false>(a, l, k * SCAN_K, h, p);
     }
@@ -208,19 +223,19 @@ __global__ __launch_bounds__(256) void plc_scan_bwd_kernel(ScanArgs a) {
 template <class T, int V, bool COUPLED, bool BACKWARD, bool FULL>
 __device__ __forceinline__ void scan_agg_block(const ScanArgs& a, const ScanLane& l, int t0, float (&A)[V], float (&S)[V]) {
     PlcVec<T, V> fr[SCAN_K], vr[SCAN_K];
-    scan_rows<T, V, FULL>(a.f, a.f_sb, a.f_st, l, t0, fr);
-    if (BACKWARD) scan_rows<T, V, FULL>(a.dy, a.dy_sb, a.dy_st, l, t0, vr);
-    else scan_rows<T, V, FULL>(a.x, a.x_sb, a.x_st, l, t0, vr);
+    scan_rows<T, V, FULL>(a, a.f, a.f_sb, a.f_st, l, t0, fr);
+    if (BACKWARD) scan_rows<T, V, FULL>(a, a.dy, a.dy_sb, a.dy_st, l, t0, vr);
+    else scan_rows<T, V, FULL>(a, a.x, a.x_sb, a.x_st, l, t0, vr);
 #pragma unroll
     for (int jj = 0; jj < SCAN_K; ++jj) {
         const int j = BACKWARD ? SCAN_K - 1 - jj : jj;
-        if (FULL || t0 + j < l.n) {
+        const bool on = FULL || t0 + j < l.n;
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float w = scan_gate<T>(fr[j].get(i)), v = vr[j].get(i), s = scan_s(w);
-                A[i] *= s;
-                S[i] = BACKWARD ? s * (v + S[i]) : scan_step<COUPLED>(S[i], v, w);
-            }
+        for (int i = 0; i < V; ++i) {
+            const float w = scan_gate<T>(fr[j].get(i)), v = vr[j].get(i), s = scan_s(w);
+            const float next = BACKWARD ? s * (v + S[i]) : scan_step<COUPLED>(S[i], v, w);
+            A[i] = on ? A[i] * s : A[i];
+            S[i] = on ? next : S[i];
         }
     }
 }
@@ -253,7 +268,7 @@ __global__ __launch_bounds__(64 * SCAN_WAVES) void plc_scan_segments_kernel(Scan
     for (int q = 0; q < blocks; ++q) {
         const int t = t0 + (BACKWARD ? blocks - 1 - q : q) * SCAN_K;
         if (__all(t + SCAN_K <= l.n)) scan_agg_block<T, V, COUPLED, BACKWARD, true>(a, l, t, A, S);
-        else scan_agg_block<T, V, COUPLED, BACKWARD, false>(a, l, t, A, S);
+        else if (__any(t < l.n)) scan_agg_block<T, V, COUPLED, BACKWARD, false>(a, l, t, A, S);
     }
     float* agg = a.agg + (long long)s.k * 2 * a.B * a.D + l.b * a.D + l.d;
     plc_store<float, V>(agg, plc_from_float<float, V>(A));
