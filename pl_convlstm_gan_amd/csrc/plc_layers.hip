@@ -82,6 +82,7 @@ static int scan_check(const plc_scan_desc* d, bool backward, ScanArgs* a, int* v
     const int e = dtype_size(d->dtype);
     PLC_REQUIRE(e, "gated scan: unknown element type %d", d->dtype);
     PLC_REQUIRE(d->B >= 0 && d->T >= 0 && d->D >= 0, "gated scan: negative size");
+    if (d->T > 1 << 30) return plc_fail(PLC_EUNSUPPORTED, "gated scan: %d steps are more than 2^30", d->T);
     memset(a, 0, sizeof(*a));
     if (d->B == 0 || d->D == 0) return PLC_OK;
     const bool any = d->T > 0;
@@ -118,10 +119,9 @@ static void scan_plan(ScanArgs* a, int vmax, bool backward, int* v) {
     a->nseg = 1;
     a->seg = a->T;
     if (n / *v / 64 < 512 && a->T >= 4 * SCAN_K) {
-        *v = vmax;
-        while (*v > 1 && n / *v < 1024) *v /= 2;
-        const long long tiles = (n / *v + 63) / 64;
-        long long want = 2048 / tiles, most = 512;
+        *v = vmax >= 2 && n >= 1024 ? 2 : 1;
+        const long long most = a->T >= 1 << 18 ? 64 * 4 * SCAN_RUN : 64 * SCAN_RUN;
+        long long want = 4096 * 64ll / (n / *v);
         want = want > most ? most : (want < 1 ? 1 : want);
         long long seg = (a->T + want - 1) / want;
         seg = (seg + SCAN_K - 1) / SCAN_K * SCAN_K;
@@ -134,13 +134,26 @@ static void scan_plan(ScanArgs* a, int vmax, bool backward, int* v) {
     }
 }
 
+template <bool BACKWARD, int R>
+static void scan_carry_runs(const ScanArgs& a, hipStream_t st) {
+    constexpr int CH = scan_carry_channels(R);
+    hipLaunchKernelGGL((plc_scan_carry_kernel<BACKWARD, R>), dim3((unsigned)(((long long)a.B * a.D + CH - 1) / CH)), dim3(R * CH), 0, st, a);
+}
+template <bool BACKWARD>
+static void scan_carry(const ScanArgs& a, hipStream_t st) {
+    if (a.nseg <= SCAN_RUN) scan_carry_runs<BACKWARD, 1>(a, st);
+    else if (a.nseg <= 4 * SCAN_RUN) scan_carry_runs<BACKWARD, 4>(a, st);
+    else if (a.nseg <= 16 * SCAN_RUN) scan_carry_runs<BACKWARD, 16>(a, st);
+    else scan_carry_runs<BACKWARD, 64>(a, st);
+}
+
 template <class T, int V, bool COUPLED, bool BACKWARD>
 static int scan_launch(const ScanArgs& a, hipStream_t st) {
     const long long lanes = a.B * (a.D / V);
     if (a.nseg > 1) {
-        const long long blocks = (lanes + 63) / 64 * cdiv(a.nseg, SCAN_WAVES);
-        const dim3 grid((unsigned)blocks), block(64 * SCAN_WAVES);
+        const dim3 grid((unsigned)((lanes * a.nseg + 255) / 256)), block(256);
         hipLaunchKernelGGL((plc_scan_segments_kernel<T, V, COUPLED, BACKWARD>), grid, block, 0, st, a);
+        scan_carry<BACKWARD>(a, st);
         hipLaunchKernelGGL((plc_scan_split_kernel<T, V, COUPLED, BACKWARD>), grid, block, 0, st, a);
     } else {
         const long long blocks = (lanes + 255) / 256;

@@ -9,7 +9,7 @@
 // Steps a lane holds in registers at a time: their loads are all requested before the first is used, and the
 // backward pass rebuilds the states of one such block from the state in front of it.
 constexpr int SCAN_K = 8;
-constexpr int SCAN_WAVES = 8;         // split form: segments (one per wave) of a workgroup
+constexpr int SCAN_RUN = 16;          // split form, carry kernel: segments a thread holds in registers
 
 struct ScanArgs {
     int B, T;
@@ -79,9 +79,10 @@ __device__ __forceinline__ void scan_load_state(const float* p, long long at, fl
 // memory of the tensor, and what is loaded there is not used.
 template <class T, int V, bool FULL>
 __device__ __forceinline__ void scan_rows(const ScanArgs& a, const void* base, long long sb, long long st, const ScanLane& l, int t0, PlcVec<T, V> (&r)[SCAN_K]) {
-    const T* p = (const T*)base + l.b * sb + l.d;
+    const T* p = (const T*)base + l.b * sb + l.d + t0 * st;
+    const int most = a.T - 1 - t0;
 #pragma unroll
-    for (int j = 0; j < SCAN_K; ++j) r[j] = plc_load<T, V>(p + (FULL ? t0 + j : min(t0 + j, a.T - 1)) * st);
+    for (int j = 0; j < SCAN_K; ++j) r[j] = plc_load<T, V>(p + (FULL ? j : min(j, most)) * st);
 }
 
 // ---- forward ----------------------------------------------------------------------------------------------------
@@ -217,9 +218,17 @@ __global__ __launch_bounds__(256) void plc_scan_bwd_kernel(ScanArgs a) {
 
 // ---- split form: few channels, many steps -----------------------------------------------------------------------
 // A segment of steps does h -> A h + S to the state (A the product of its gates), and the same to the gradient that runs
-// backwards, p -> A p + S.  The first launch computes A and S of every segment (one wave per segment and 64 lanes), the
-// second folds those in front of (behind) its segment into the state it starts from and walks the segment as above.  x and f
-// (f and dy) are read twice, the second time mostly from the cache; in return every segment runs at once.
+// backwards, p -> A p + S.  The first launch computes A and S of every segment, the second turns them into the state in
+// front of (the gradient behind) each, the third walks the segments as above.  x and f (f and dy) are read twice, the second
+// time mostly from the cache; in return every segment runs at once.  Lanes run over (segment, channels): a row of few
+// channels does not leave lanes of a wave idle, and a lane keeps the widest access.
+template <int V>
+__device__ __forceinline__ bool scan_item(const ScanArgs& a, ScanLane& l, int& k) {
+    const unsigned lanes = (unsigned)(a.B * (a.D / V)), i = blockIdx.x * blockDim.x + threadIdx.x;
+    k = (int)(i / lanes);
+    return k < a.nseg && scan_lane<V>(a, i - (unsigned)k * lanes, l);
+}
+
 template <class T, int V, bool COUPLED, bool BACKWARD, bool FULL>
 __device__ __forceinline__ void scan_agg_block(const ScanArgs& a, const ScanLane& l, int t0, float (&A)[V], float (&S)[V]) {
     PlcVec<T, V> fr[SCAN_K], vr[SCAN_K];
@@ -240,109 +249,89 @@ __device__ __forceinline__ void scan_agg_block(const ScanArgs& a, const ScanLane
     }
 }
 
-// workgroup: SCAN_WAVES segments of 64 lanes; blockIdx.x = group of segments + number of groups * tile of lanes
-struct ScanSeg {
-    int first, k, wave, lane;       // first segment of the workgroup, this wave's, ...
-    long long i;
-};
-__device__ __forceinline__ ScanSeg scan_seg(const ScanArgs& a) {
-    ScanSeg s;
-    const unsigned groups = (a.nseg + SCAN_WAVES - 1) / SCAN_WAVES, tile = blockIdx.x / groups;
-    s.wave = threadIdx.x >> 6;
-    s.lane = threadIdx.x & 63;
-    s.first = (int)(blockIdx.x - tile * groups) * SCAN_WAVES;
-    s.k = s.first + s.wave;
-    s.i = (long long)tile * 64 + s.lane;
-    return s;
-}
-
 template <class T, int V, bool COUPLED, bool BACKWARD>
-__global__ __launch_bounds__(64 * SCAN_WAVES) void plc_scan_segments_kernel(ScanArgs a) {
-    const ScanSeg s = scan_seg(a);
+__global__ __launch_bounds__(256) void plc_scan_segments_kernel(ScanArgs a) {
     ScanLane l;
-    if (s.k >= a.nseg || !scan_lane<V>(a, s.i, l)) return;
+    int k;
+    if (!scan_item<V>(a, l, k)) return;
     float A[V], S[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) A[i] = 1.0f, S[i] = 0.0f;
-    const int t0 = s.k * a.seg, t1 = min(t0 + a.seg, a.T), blocks = (t1 - t0 + SCAN_K - 1) / SCAN_K;
+    const int t0 = k * a.seg, t1 = min(t0 + a.seg, a.T), blocks = (t1 - t0 + SCAN_K - 1) / SCAN_K;
     for (int q = 0; q < blocks; ++q) {
         const int t = t0 + (BACKWARD ? blocks - 1 - q : q) * SCAN_K;
         if (__all(t + SCAN_K <= l.n)) scan_agg_block<T, V, COUPLED, BACKWARD, true>(a, l, t, A, S);
         else if (__any(t < l.n)) scan_agg_block<T, V, COUPLED, BACKWARD, false>(a, l, t, A, S);
     }
-    float* agg = a.agg + (long long)s.k * 2 * a.B * a.D + l.b * a.D + l.d;
+    float* agg = a.agg + (long long)k * 2 * a.B * a.D + l.b * a.D + l.d;
     plc_store<float, V>(agg, plc_from_float<float, V>(A));
     plc_store<float, V>(agg + (long long)a.B * a.D, plc_from_float<float, V>(S));
 }
 
-// (A, S) after segments k0, k0 + step, ... (count of them)
-template <int V>
-__device__ __forceinline__ void scan_fold(const float* agg, long long n, long long stride, int count, float (&A)[V], float (&S)[V]) {
-    constexpr int U = 8;
-    for (int q = 0; q < count; q += U) {
-        PlcVec<float, V> ra[U], rs[U];
+// (A, S) of the segments -> what each starts from, in A's place.  R threads per channel, each a run of segments: folded, the
+// runs joined in order through LDS, walked again.  A run of up to SCAN_RUN segments is read once and kept (the launch picks
+// R for that; only more than 64 * SCAN_RUN segments are read twice).
+constexpr int scan_carry_channels(int R) { return R == 64 ? 16 : 256 / R; }
+
+template <bool BACKWARD, int R>
+__global__ __launch_bounds__(R * scan_carry_channels(R)) void plc_scan_carry_kernel(ScanArgs a) {
+    constexpr int CH = scan_carry_channels(R);
+    __shared__ float part[2][R][CH];
+    const int ch = threadIdx.x % CH, run = threadIdx.x / CH;
+    const long long n = (long long)a.B * a.D, c = (long long)blockIdx.x * CH + ch;
+    const int share = (a.nseg + R - 1) / R, q0 = min(run * share, a.nseg), q1 = min(q0 + share, a.nseg);
+    float* agg = a.agg + c;
+    auto at = [&](int q) { return (long long)(BACKWARD ? a.nseg - 1 - q : q) * 2 * n; };
+    float A = 1.0f, S = 0.0f, ra[SCAN_RUN], rs[SCAN_RUN];
+    auto load = [&](int q) {
 #pragma unroll
-        for (int j = 0; j < U; ++j)
-            if (q + j < count) {
-                ra[j] = plc_load<float, V>(agg + (q + j) * stride);
-                rs[j] = plc_load<float, V>(agg + (q + j) * stride + n);
-            }
+        for (int j = 0; j < SCAN_RUN; ++j)
+            if (q + j < q1) ra[j] = agg[at(q + j)], rs[j] = agg[at(q + j) + n];
+    };
+    if (c < n)
+        for (int q = q0; q < q1; q += SCAN_RUN) {
+            load(q);
 #pragma unroll
-        for (int j = 0; j < U; ++j)
-            if (q + j < count) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    S[i] = __builtin_fmaf(ra[j].get(i), S[i], rs[j].get(i));
-                    A[i] *= ra[j].get(i);
+            for (int j = 0; j < SCAN_RUN; ++j)
+                if (q + j < q1) {
+                    S = __builtin_fmaf(ra[j], S, rs[j]);
+                    A *= ra[j];
                 }
+        }
+    if (R > 1) {
+        part[0][run][ch] = A;
+        part[1][run][ch] = S;
+        __syncthreads();
+    }
+    if (c >= n) return;
+    const float* first = BACKWARD ? a.dh_last : a.h0;
+    float h = first ? first[c] : 0.0f;
+#pragma unroll 8
+    for (int r = 0; r < run; ++r) h = __builtin_fmaf(part[0][r][ch], h, part[1][r][ch]);
+    for (int q = q0; q < q1; q += SCAN_RUN) {
+        if (share > SCAN_RUN) load(q);
+#pragma unroll
+        for (int j = 0; j < SCAN_RUN; ++j)
+            if (q + j < q1) {
+                agg[at(q + j)] = h;
+                h = __builtin_fmaf(ra[j], h, rs[j]);
             }
     }
 }
 
 template <class T, int V, bool COUPLED, bool BACKWARD>
-__global__ __launch_bounds__(64 * SCAN_WAVES) void plc_scan_split_kernel(ScanArgs a) {
-    __shared__ float part[2][SCAN_WAVES][64 * V];
-    const ScanSeg s = scan_seg(a);
+__global__ __launch_bounds__(256) void plc_scan_split_kernel(ScanArgs a) {
     ScanLane l;
-    const bool on = scan_lane<V>(a, s.i, l);
-    const long long n = (long long)a.B * a.D, per = 2 * n;
-    // the segments outside the workgroup that come first (forward: in front of it, backward: behind it), an equal share to
-    // each wave, joined in order through LDS
-    const int last = min(s.first + SCAN_WAVES, a.nseg);               // one behind the workgroup's segments
-    const int before = BACKWARD ? a.nseg - last : s.first;
-    const int share = (before + SCAN_WAVES - 1) / SCAN_WAVES;
-    const int q0 = min(s.wave * share, before), q1 = min(q0 + share, before);
-    float A[V], S[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) A[i] = 1.0f, S[i] = 0.0f;
-    const float* agg = a.agg + l.b * a.D + l.d;
-    if (on && q1 > q0) {
-        if (BACKWARD) scan_fold<V>(agg + (a.nseg - 1 - q0) * per, n, -per, q1 - q0, A, S);
-        else scan_fold<V>(agg + q0 * per, n, per, q1 - q0, A, S);
-    }
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        part[0][s.wave][s.lane * V + i] = A[i];
-        part[1][s.wave][s.lane * V + i] = S[i];
-    }
-    __syncthreads();
-    if (!on || s.k >= a.nseg) return;
+    int k;
+    if (!scan_item<V>(a, l, k)) return;
     float h[V];
-    scan_load_state<V>(BACKWARD ? a.dh_last : a.h0, l.b * a.D + l.d, h);
-    for (int q = 0; q < SCAN_WAVES; ++q)
-#pragma unroll
-        for (int i = 0; i < V; ++i) h[i] = __builtin_fmaf(part[0][q][s.lane * V + i], h[i], part[1][q][s.lane * V + i]);
-    float one[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) one[i] = 1.0f;
-    const int t0 = s.k * a.seg, t1 = min(t0 + a.seg, a.T);
+    scan_load_state<V>(a.agg, (long long)k * 2 * a.B * a.D + l.b * a.D + l.d, h);
+    const int t0 = k * a.seg, t1 = min(t0 + a.seg, a.T);
     if (BACKWARD) {
-        scan_fold<V>(agg + (last - 1) * per, n, -per, last - 1 - s.k, one, h);
         scan_bwd_range<T, V, COUPLED>(a, l, t0, t1, h);
-        if (s.k == 0 && a.dh0) plc_store<float, V>(a.dh0 + l.b * a.D + l.d, plc_from_float<float, V>(h));
+        if (k == 0 && a.dh0) plc_store<float, V>(a.dh0 + l.b * a.D + l.d, plc_from_float<float, V>(h));
     } else {
-        scan_fold<V>(agg + s.first * per, n, per, s.wave, one, h);
         scan_fwd_range<T, V, COUPLED>(a, l, t0, t1, h);
-        if (s.k == a.nseg - 1 && a.h_last) plc_store<float, V>(a.h_last + l.b * a.D + l.d, plc_from_float<float, V>(h));
+        if (k == a.nseg - 1 && a.h_last) plc_store<float, V>(a.h_last + l.b * a.D + l.d, plc_from_float<float, V>(h));
     }
 }
