@@ -216,6 +216,28 @@ def lib():
     return L
 
 
+_binding = None
+
+
+def binding():
+    """The native PyTorch binding of the layer operators (csrc/plc_torch.cpp, built as _plc_torch.so beside the
+    library), calling the library that lib() has loaded."""
+    global _binding
+    if _binding is None:
+        L = lib()
+        try:
+            from . import _plc_torch as m
+        except ImportError as e:
+            raise RuntimeError("the PyTorch binding of the layer operators (_plc_torch.so) does not load: "
+                               f"{e} (run `python -c 'import __graft_entry__ as g; g.build()'`)") from e
+        if m.abi_version != ABI_VERSION:
+            raise RuntimeError(f"_plc_torch.so is version {m.abi_version} of the C ABI, this package is version {ABI_VERSION}: rebuild it")
+        m.bind({name: C.cast(getattr(L, name), C.c_void_p).value for name in EXPORTS
+                if name == "plc_last_error" or name.startswith(("plc_gated_scan", "plc_group_norm", "plc_dropout"))})
+        _binding = m
+    return _binding
+
+
 def check(rc: int, what: str):
     """Raise with the library's message if a call returned an error code."""
     if rc != 0:

@@ -9,33 +9,8 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
-from . import ops
-
-
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
-
-
-# ------------------------------------------------------------------------------------ gated linear recurrence
-class _ScanFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, f, h0, lengths, coupled):
-        y, h_last, states = ops.gated_scan_forward(x, f, h0, lengths, coupled, save_states=True)
-        ctx.save_for_backward(x, f, h0, lengths, states)
-        ctx.coupled = coupled
-        ctx.set_materialize_grads(False)
-        return y, h_last
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dh_last):
-        x, f, h0, lengths, states = ctx.saved_tensors
-        if dy is None and dh_last is None:
-            return (None,) * 5
-        dx, df, dh0 = ops.gated_scan_backward(x, f, h0, lengths, ctx.coupled, states, dy, dh_last, ctx.needs_input_grad[2])
-        return dx, df, dh0, None, None
+from . import _lib, ops
 
 
 def gated_linear_scan(x, f, h0=None, lengths=None, coupled=True):
@@ -45,43 +20,13 @@ def gated_linear_scan(x, f, h0=None, lengths=None, coupled=True):
     ``h0``: float32 [B, ...], the state in front of the first step (default zeros).  ``lengths``: int32 [B] on x's
     device; behind a sample's length the outputs and gradients are 0, whatever the padding holds, and its state stands
     still.  Strided x and f are read in place as long as their trailing dimensions are contiguous."""
-    if _wants_grad(x, f, h0):
-        return _ScanFn.apply(x, f, h0, lengths, bool(coupled))
-    return ops.gated_scan_forward(x, f, h0, lengths, coupled)[:2]
+    return _lib.binding().scan(x, f, h0, lengths, coupled)
 
 
 def gated_linear_step(x, f, state, coupled=True, inplace=False):
     """One step of gated_linear_scan for serving, without gradients: x, f [B, ...], ``state`` float32 [B, ...];
     returns (h in x's type, new state).  ``inplace``: the new state overwrites ``state``."""
-    x, f = (ops._require_layer(t, n).detach() for t, n in ((x, "x"), (f, "f")))
-    state = ops._require_layer(state, "state", x, torch.float32).detach()
-    if inplace and not state.is_contiguous():
-        raise ValueError("a state that is updated in place must be contiguous")
-    y, new, _ = ops.gated_scan_forward(x.unsqueeze(1), f.unsqueeze(1), state, None, coupled, h_last=state if inplace else None)
-    return y.squeeze(1), new
-
-
-# ------------------------------------------------------------------------------------ dropout
-def _used_offset(offset):
-    return torch.empty_like(offset) if isinstance(offset, torch.Tensor) else None
-
-
-class _DropoutFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, p, seed, offset):
-        used = _used_offset(offset)
-        y = ops.dropout_forward(x, p, seed, offset, residual, used)
-        ctx.args = (p, seed, None if used is not None else offset)
-        ctx.save_for_backward(used)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        (used,) = ctx.saved_tensors
-        p, seed, offset = ctx.args
-        dx = ops.dropout_forward(dy, p, seed, used if used is not None else offset) if ctx.needs_input_grad[0] else None
-        return dx, (dy if ctx.needs_input_grad[1] else None), None, None, None
+    return _lib.binding().step(x, f, state, coupled, inplace)
 
 
 def counter_dropout(x, p, seed, offset=0, residual=None):
@@ -92,29 +37,8 @@ def counter_dropout(x, p, seed, offset=0, residual=None):
     Calls that must not share a mask take different offsets.  ``offset`` is an integer or an int64 tensor of one element on
     x's device that the kernel reads when it runs: a captured graph that advances it draws a new mask on every replay
     (the backward pass keeps the value its forward pass used)."""
-    if _wants_grad(x, residual):
-        return _DropoutFn.apply(x, residual, p, seed, offset)
-    return ops.dropout_forward(x, p, seed, offset, residual)
-
-
-# ------------------------------------------------------------------------------------ group norm
-class _NormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, groups, eps, act, p, seed, offset):
-        used = _used_offset(offset) if p > 0 else None
-        y, stats = ops.group_norm_forward(x, groups, weight, bias, eps, act, p, seed, offset, used)
-        ctx.args = (groups, eps, act, p, seed, None if used is not None else offset)
-        ctx.save_for_backward(x, weight, bias, stats, used)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias, stats, used = ctx.saved_tensors
-        groups, eps, act, p, seed, offset = ctx.args
-        dx, dw, db = ops.group_norm_backward(x, groups, weight, bias, eps, act, p, seed, used if used is not None else offset,
-                                             stats, dy)
-        return dx, dw, db, None, None, None, None, None, None
+    seed, offset, offset_t = ops._draw(seed, offset)
+    return _lib.binding().dropout(x, p, seed, offset, offset_t, residual)
 
 
 def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", p=0.0, seed=0, offset=0):
@@ -122,9 +46,8 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
     pass.  ``weight`` and ``bias``: float32 [C] or None.  x is taken channels last in memory (another layout is copied into
     it first) and the result is channels last.  ``seed`` and ``offset`` as in counter_dropout; elements are counted in
     [N, H, W, C] order."""
-    if _wants_grad(x, weight, bias):
-        return _NormFn.apply(x, weight, bias, num_groups, float(eps), act, float(p), seed, offset)
-    return ops.group_norm_forward(x, num_groups, weight, bias, eps, act, p, seed, offset)[0]
+    seed, offset, offset_t = ops._draw(seed, offset)
+    return _lib.binding().norm(x, num_groups, weight, bias, eps, ops._act(act), p, seed, offset, offset_t)
 
 
 class GroupNormAct(nn.Module):
