@@ -189,6 +189,15 @@ typedef struct plc_rollout_desc {
     /* caller-owned scratch of plc_generator_workspace_bytes(desc) bytes, 256-byte aligned */
     void* workspace;
     size_t workspace_bytes;
+    /* Feature head (not in the reference; head_groups = 0: none, the reference's model): the features h2_t of every
+     * frame go through group norm, an activation and, for head_p > 0, dropout (plc_group_norm_fwd) before the upsample blocks.
+     * C2 must be a multiple of 8 and of head_groups. */
+    int head_groups, head_act;
+    float head_eps;
+    double head_p;
+    unsigned long long head_seed;
+    const long long* head_offset;   /* device int64, read when the forward pass runs (NULL: 0); the backward pass uses the value it read */
+    const float* head_w; const float* head_b;   /* [C2] or NULL */
 } plc_rollout_desc;
 
 size_t plc_generator_workspace_bytes(const plc_rollout_desc* d);
@@ -281,6 +290,8 @@ typedef struct plc_rollout_grads {
     float* d_rain;           /* [B][T][1][H][W] */
     float* d_dem;            /* [B][1][dem_H][dem_W] */
     float* d_lu;             /* [B][L][lu_H][lu_W] */
+    /* gradients of the feature head's weight and bias ([C2], overwritten; NULL = not wanted) */
+    float* head_w; float* head_b;
 } plc_rollout_grads;
 
 size_t plc_generator_bwd_workspace_bytes(const plc_rollout_desc* d);

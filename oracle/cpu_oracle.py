@@ -145,13 +145,14 @@ def attention_gate(aux, w0, b0, w1, b1, emulate: Optional[str] = None):
 # --------------------------------------------------------------------------------------
 def generator_forward(p: Params, rain_lr, dem, lu, *, scale_factor=None, target_grid_size=None,
                       input_grid_size=None, emulate: Optional[str] = None,
-                      return_states: bool = False):
+                      return_states: bool = False, feature_head=None):
     """Whole rollout.  rain_lr [B,T,1,H,W], dem [B,1,.,.], lu [B,L,.,.] -> [B,T,1,Hh,Wh].
 
     The two attention gates do not depend on t, so they are evaluated once and their
     product is applied every step (generator.py:198-199 evaluates them inside the loop;
     the values are identical).  The number of upsample blocks is read from the params
     dict (they must have been materialised, generator.py:129-132).
+    ``feature_head(h2, t)``: what the engine's optional feature head does to the features of step t (not in the reference).
     """
     q = _q(emulate)
     B, T, _, H, W = rain_lr.shape
@@ -190,7 +191,7 @@ def generator_forward(p: Params, rain_lr, dem, lu, *, scale_factor=None, target_
         h2 = q(h2)
         if return_states:
             states.append((h1, c1, h2, c2))
-        feat = h2
+        feat = h2 if feature_head is None else q(feature_head(h2, t))
         for k in range(n_blocks):
             w = p[f"upsample_blocks.{k}.conv.weight"]
             b = p[f"upsample_blocks.{k}.conv.bias"]

@@ -51,6 +51,8 @@ class RolloutDesc(C.Structure):
         ("up_w", _f * 8), ("up_b", _f * 8),
         ("post0_w", _f), ("post0_b", _f), ("post2_w", _f), ("post2_b", _f),
         ("out", _f), ("workspace", _f), ("workspace_bytes", C.c_size_t),
+        ("head_groups", C.c_int), ("head_act", C.c_int), ("head_eps", C.c_float), ("head_p", C.c_double),
+        ("head_seed", C.c_ulonglong), ("head_offset", _f), ("head_w", _f), ("head_b", _f),
     ]
 
 
@@ -64,7 +66,7 @@ class RolloutGrads(C.Structure):
         ("up_w", _f * 8), ("up_b", _f * 8),
         ("post0_w", _f), ("post0_b", _f), ("post2_w", _f), ("post2_b", _f),
         ("workspace", _f), ("workspace_bytes", C.c_size_t),
-        ("d_rain", _f), ("d_dem", _f), ("d_lu", _f),
+        ("d_rain", _f), ("d_dem", _f), ("d_lu", _f), ("head_w", _f), ("head_b", _f),
     ]
 
 

@@ -40,6 +40,8 @@ def _param_list(model):
         ps += [blk.conv.weight, blk.conv.bias]
     ps += [model.post_process[0].weight, model.post_process[0].bias,
            model.post_process[2].weight, model.post_process[2].bias]
+    if model.feature_norm is not None:
+        ps += [model.feature_norm.weight, model.feature_norm.bias]
     return ps
 
 
@@ -52,6 +54,7 @@ class _RolloutFn(torch.autograd.Function):
         ctx.ws = ws                      # saved activations live in the forward workspace (+ the bound parameters)
         ctx.keep = (rain_lr, dem, lu)    # the descriptor holds raw pointers into these
         ctx.n_blocks = len(model.upsample_blocks)
+        ctx.head = model.feature_norm is not None
         ctx.shapes = [p.shape for p in params]
         return out
 
@@ -77,6 +80,8 @@ class _RolloutFn(torch.autograd.Function):
             g.up_w[k], g.up_b[k] = nxt(), nxt()
         g.post0_w, g.post0_b = nxt(), nxt()
         g.post2_w, g.post2_b = nxt(), nxt()
+        if ctx.head:
+            g.head_w, g.head_b = nxt(), nxt()
         nbytes = L.plc_generator_bwd_workspace_bytes(C.byref(d))
         if nbytes == 0:
             msg = L.plc_last_error().decode("utf-8", "replace")

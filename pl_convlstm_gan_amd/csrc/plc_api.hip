@@ -886,6 +886,9 @@ struct RolloutPlan {
     size_t mid, fin;    // after residual resize / after target resize (== previous stage if unused)
     size_t dem_hr, lu_hr, dem_mid, lu_mid, gate_dem, gate_lu, gate, p0;
     size_t sync;        // the persistent recurrence kernel's barrier counter
+    // feature head (desc.head_groups > 0): its output (the features everything after the recurrence reads), statistics,
+    // the dropout offset the forward pass used, workspace
+    size_t head, head_stats, head_used, head_ws, head_ws_bytes;
     // fp8 gate convs (desc.gate_fp8): fp8 copies of the cells' operands, fp8 weight fragments, scale words
     size_t xs8, h1s8, h2s8, cell1_w8, cell2_w8, scale8;
     size_t total;
@@ -893,6 +896,25 @@ struct RolloutPlan {
     int up_H, up_W;     // size after the PixelShuffle blocks
     size_t img1, img2;  // bytes of one CB8 bf16 image of C1 / C2 channels at LR size
 };
+
+// The feature head as a group norm over the T * B frames of h2; x, y, ... are filled in by the callers.
+static plc_norm_desc head_desc(const plc_rollout_desc* d) {
+    plc_norm_desc n;
+    memset(&n, 0, sizeof(n));
+    n.N = d->T * d->B;
+    n.C = d->C2;
+    n.G = d->head_groups;
+    n.HW = d->H * d->W;
+    n.dtype = PLC_BF16;
+    n.layout = PLC_CB8;
+    n.act = d->head_act;
+    n.eps = d->head_eps;
+    n.weight = d->head_w;
+    n.bias = d->head_b;
+    n.p = d->head_p;
+    n.seed = d->head_seed;
+    return n;
+}
 
 static int rollout_plan(const plc_rollout_desc* d, RolloutPlan* p) {
     PLC_REQUIRE(d, "rollout: null descriptor");
@@ -942,6 +964,20 @@ static int rollout_plan(const plc_rollout_desc* d, RolloutPlan* p) {
         p->gates1 = p->gates2 = (size_t)-1;
     }
     size_t cur = p->h2s + (size_t)B * p->img2;  // h2_0 .. h2_{T-1}
+    p->head = p->head_stats = p->head_used = p->head_ws = (size_t)-1;
+    p->head_ws_bytes = 0;
+    if (d->head_groups != 0) {
+        PLC_REQUIRE(d->head_groups > 0 && R2 % d->head_groups == 0, "rollout: %d features do not divide into %d groups", R2, d->head_groups);
+        if (R2 % 8) return plc_fail(PLC_EUNSUPPORTED, "rollout: the feature head takes whole blocks of 8 features, not %d", R2);
+        const plc_norm_desc n = head_desc(d);
+        p->head_ws_bytes = plc_group_norm_workspace_bytes(&n, 0);
+        if (p->head_ws_bytes == 0) return PLC_EINVAL;          // (the message is the group norm's)
+        p->head = take((size_t)T * B * p->img2);
+        p->head_stats = take((size_t)T * B * d->head_groups * 2 * sizeof(float));
+        p->head_used = take(sizeof(long long));
+        p->head_ws = take(p->head_ws_bytes);
+        cur = p->head;
+    }
     for (int k = 0; k < d->n_blocks; ++k) {
         const size_t s = (size_t)(d->H << (k + 1)) * (d->W << (k + 1));
         p->up_out[k] = take((size_t)T * B * (C2 / 8) * s * 16);
@@ -999,6 +1035,7 @@ extern "C" size_t plc_generator_workspace_offset(const plc_rollout_desc* d, cons
     if (!strcmp(name, "gate")) return p.gate;
     if (!strcmp(name, "p0")) return p.p0;
     if (!strcmp(name, "feat")) return p.fin;
+    if (!strcmp(name, "head")) return p.head;
     return (size_t)-1;
 }
 
@@ -1268,6 +1305,18 @@ extern "C" int plc_generator_rollout_fwd(const plc_rollout_desc* d, void* stream
     // ---- everything after the recurrence is batched over the T*B frames ----------------------
     const int NI = T * B;
     const char* feat = ws + p.h2s + (size_t)B * p.img2;
+    if (d->head_groups) {
+        plc_norm_desc n = head_desc(d);
+        n.x = feat;
+        n.y = ws + p.head;
+        n.stats = (float*)(ws + p.head_stats);
+        n.offset_ptr = d->head_offset;
+        n.used_offset = (long long*)(ws + p.head_used);
+        n.workspace = ws + p.head_ws;
+        n.workspace_bytes = p.head_ws_bytes;
+        if ((rc = plc_group_norm_fwd(&n, st))) return rc;
+        feat = ws + p.head;
+    }
     int fh = H, fw = W;
     for (int k = 0; k < d->n_blocks; ++k) {
         ConvArgs a = conv_args(fh, fw, NI);

@@ -539,6 +539,7 @@ struct BwdPlan {
     size_t d_conv[8], d_in[8];
     size_t d_mid, d_up;     // (size_t)-1 when the corresponding bilinear resize is absent
     size_t dz1, dz2, dcat1, dcat2, dc1, dc2, slab, slab_bytes, total;
+    size_t d_head, head_ws, head_ws_bytes;      // feature head: gradient of h2, workspace
 };
 
 static size_t max_sz(size_t a, size_t b) { return a > b ? a : b; }
@@ -598,6 +599,14 @@ static int bwd_plan(const plc_rollout_desc* d, const RolloutPlan& fp, BwdPlan* p
     if (!widths_fast(C1, C2)) sb += 4 * max_sz(wgrad_slab_bytes<4, 0, 4, 3>(), wgrad_slab_bytes<4, 0, 4, 1>());
     p->slab_bytes = sb;
     p->slab = take(sb);
+    p->d_head = p->head_ws = (size_t)-1;
+    p->head_ws_bytes = 0;
+    if (d->head_groups) {
+        const plc_norm_desc n = head_desc(d);
+        p->head_ws_bytes = plc_group_norm_workspace_bytes(&n, 1);
+        p->d_head = take((size_t)NI * (C2 / 8) * hw * 16);
+        p->head_ws = take(p->head_ws_bytes);
+    }
     p->total = o;
     (void)T;
     return PLC_OK;
@@ -733,7 +742,8 @@ extern "C" int plc_generator_rollout_bwd(const plc_rollout_desc* d, const plc_ro
     // of the gated feature map IS cell 2's incoming dh: its pointwise backward then forms
     // d_feat * gate itself (the gate is one image per batch element, cache-resident) and the
     // T*B-image product is neither written by the gate backward nor read back.
-    const bool direct = d->n_blocks == 0 && bp.d_mid == (size_t)-1 && bp.d_up == (size_t)-1;
+    // (Not with a feature head, which takes the product itself.)
+    const bool direct = d->n_blocks == 0 && bp.d_mid == (size_t)-1 && bp.d_up == (size_t)-1 && !d->head_groups;
     // ---- gating and the two attention branches ------------------------------------------------
     {
         GateBwdArgs ga;
@@ -834,7 +844,7 @@ extern "C" int plc_generator_rollout_bwd(const plc_rollout_desc* d, const plc_ro
     for (int k = d->n_blocks - 1; k >= 0; --k) {
         const int kh = H << k, kw = W << k;
         const long long khw = (long long)kh * kw;
-        const char* in_k = (k == 0) ? wf + fp.h2s + (size_t)B * fp.img2 : wf + fp.up_out[k - 1];
+        const char* in_k = k > 0 ? wf + fp.up_out[k - 1] : d->head_groups ? wf + fp.head : wf + fp.h2s + (size_t)B * fp.img2;
         hipLaunchKernelGGL(plc_pixel_unshuffle_mask_kernel, dim3(ew_grid((long long)NI * (C2 / 8) * khw)), dim3(256),
                            0, st, cur, (const char*)(wf + fp.up_out[k]), wb + bp.d_conv[k], NI, C2, kh, kw);
         PLC_HIP(hipGetLastError());
@@ -859,6 +869,21 @@ extern "C" int plc_generator_rollout_bwd(const plc_rollout_desc* d, const plc_ro
                        : launch_convg<3, STAGE_CB8, EPI_ACT_CB8>(a, 4 * C2 / 8, 0, cdiv(C2, 32), NI, st)))
             return rc;
         cur = wb + bp.d_in[k];
+    }
+    // ---- feature head: back to the gradient of h2 ----------------------------------------------
+    if (d->head_groups) {
+        plc_norm_desc n = head_desc(d);
+        n.x = wf + fp.h2s + (size_t)B * fp.img2;
+        n.stats = (float*)(wf + fp.head_stats);
+        n.offset_ptr = (const long long*)(wf + fp.head_used);
+        n.dy = cur;
+        n.dx = wb + bp.d_head;
+        n.dweight = g->head_w;
+        n.dbias = g->head_b;
+        n.workspace = wb + bp.head_ws;
+        n.workspace_bytes = bp.head_ws_bytes;
+        if ((rc = plc_group_norm_bwd(&n, st))) return rc;
+        cur = wb + bp.d_head;
     }
     // ---- backpropagation through time ---------------------------------------------------------
     const size_t s1 = (size_t)B * fp.img1, s2 = (size_t)B * fp.img2;      // bytes of one step (bf16 CB8)

@@ -34,6 +34,10 @@ class ModelConfig:
     scale_factor: int = 8
     target_grid_size: Optional[List[int]] = None
     input_grid_size: Optional[List[int]] = None
+    # not in the reference (Generator.set_feature_head): groups of the norm on the features (0: none), activation, dropout
+    feature_groups: int = 0
+    feature_act: str = "silu"
+    feature_dropout: float = 0.0
 
 
 @dataclass
@@ -91,8 +95,11 @@ class Config:
         if parent:
             os.makedirs(parent, exist_ok=True)
         with open(yaml_path, "w", encoding="utf-8") as fh:
-            yaml.dump({name: asdict(getattr(self, name)) for name, _ in _SECTIONS}, fh,
-                      default_flow_style=False, allow_unicode=True)
+            raw = {name: asdict(getattr(self, name)) for name, _ in _SECTIONS}
+            if not raw["model"]["feature_groups"]:        # (a file without the head stays one that the reference reads)
+                for key in ("feature_groups", "feature_act", "feature_dropout"):
+                    del raw["model"][key]
+            yaml.dump(raw, fh, default_flow_style=False, allow_unicode=True)
 
     def validate(self):
         for key, value in asdict(self.data).items():

@@ -134,8 +134,30 @@ class Generator(nn.Module):
         # operand type of the two gate convolutions: "bf16", or "fp8" (e4m3 operands on the block-scaled
         # matrix instruction; hidden_dims [16,32] only).  Not a constructor argument: the reference has none.
         self.gate_dtype = "bf16"
+        self.feature_norm = None
         self._ws = {}
         self._tabs = {}
+
+    def set_feature_head(self, num_groups, act="silu", p=0.0, seed=0):
+        """Adds group norm + activation (+ dropout of probability ``p`` in training mode) on the recurrence's features, in front
+        of the upsample blocks.  Not a constructor argument: the reference has none, and without this call the model, its
+        parameters and its state_dict are the reference's.  To be called before an optimizer takes the parameters; the head's own
+        are ``feature_norm.weight`` and ``feature_norm.bias``.  ``num_groups`` = 0 removes it."""
+        if num_groups == 0:
+            self.feature_norm = None
+            return self
+        ch = int(self.hidden_dims[1])
+        if ch % 8:
+            raise NotImplementedError(f"the feature head takes whole blocks of 8 features, not {ch}")
+        if num_groups < 0 or ch % num_groups:
+            raise ValueError(f"{ch} features do not divide into {num_groups} groups")
+        ops._act(act)
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"p must be a probability (got {p})")
+        ops._draw(seed, 0)
+        from .layers import GroupNormAct
+        self.feature_norm = GroupNormAct(num_groups, ch, act, p, seed=seed).to(self.init_conv.weight.device)
+        return self
 
     # generator.py:73-92
     def _setup_upsample_blocks(self, scale_factor, device):
@@ -222,6 +244,10 @@ class Generator(nn.Module):
         if self.gate_dtype not in ("bf16", "fp8"):
             raise ValueError(f"gate_dtype must be 'bf16' or 'fp8', not {self.gate_dtype!r}")
         d.gate_fp8 = 1 if self.gate_dtype == "fp8" else 0
+        head = self.feature_norm
+        if head is not None:
+            d.head_groups, d.head_act, d.head_eps = head.num_groups, ops._act(head.act), head.eps
+            d.head_p, d.head_seed = (head.p if head.training else 0.0), head.seed
         return d, (fH, fW)
 
     def _bind(self, d, rain_lr, dem, lu, out, params):
@@ -244,6 +270,12 @@ class Generator(nn.Module):
             d.up_w[k], d.up_b[k] = P(), P()
         d.post0_w, d.post0_b = P(), P()
         d.post2_w, d.post2_b = P(), P()
+        if self.feature_norm is not None:
+            d.head_w, d.head_b = P(), P()
+            if d.head_p > 0:
+                offset = self.feature_norm.offset.to(rain_lr.device)
+                d.head_offset = offset.data_ptr()
+                keep.append(offset)
         d.out = out.data_ptr()
         return keep
 
@@ -310,6 +342,8 @@ class Generator(nn.Module):
             out = rollout_with_grad(self, rain_lr, dem, lu, input_grid_size, params)
         else:
             out = self._forward_impl(rain_lr, dem, lu, input_grid_size, False, [p.detach() for p in params])[0]
+        if self.feature_norm is not None and self.feature_norm.training and self.feature_norm.p > 0:
+            self.feature_norm.offset.add_(1)          # (on the device: a captured step draws a new mask on every replay)
         return out if out.device == home else out.to(home)
 
     def _forward_impl(self, rain_lr, dem, lu, input_grid_size, save_for_backward, params):

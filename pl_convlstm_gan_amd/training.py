@@ -325,6 +325,7 @@ class GraphedTrainStep:
         if not all(t.is_cuda for t in self.static):
             raise RuntimeError("GraphedTrainStep: the batch must be on the GPU")
         params = [p.detach().clone() for p in model.parameters()]
+        buffers = [b.detach().clone() for b in model.buffers()]      # (the dropout offset of a feature head)
         had_state = optimizer.snapshot()
         # Parameters the optimizer does not own (the reference never registers the lazily created upsample
         # blocks) are not touched by its zero_grad(): their .grad ACCUMULATES from step to step and counts in
@@ -339,6 +340,8 @@ class GraphedTrainStep:
         with torch.no_grad():
             for p, s in zip(model.parameters(), params):      # (the lazy blocks created by the warm-up keep their values)
                 p.copy_(s)
+            for b, s in zip(model.buffers(), buffers):
+                b.copy_(s)
         optimizer.restore_(had_state)
         owned = {id(p) for group in optimizer.param_groups for p in group["params"]}
         with torch.no_grad():

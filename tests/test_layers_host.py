@@ -145,3 +145,40 @@ def test_no_packed_fp32_in_any_code_object(tmp_path):
         names += dis
         assert not re.search(r"\bv_pk_(fma|mul|add)_f32\b", dis)
     assert "plc_scan_fwd_kernel" in names and "plc_lstm_pair_kernel" in names
+
+
+def test_feature_head_interface(tmp_path):
+    """Generator.set_feature_head without a GPU: parameters, refusals, configuration."""
+    from pl_convlstm_gan_amd import Generator
+    from pl_convlstm_gan_amd.host.config import Config
+    m = Generator(hidden_dims=[16, 32], lu_channels=5, scale_factor=1)
+    keys = set(m.state_dict())
+    assert m.set_feature_head(8, "relu", 0.1, seed=3) is m
+    assert set(m.state_dict()) - keys == {"feature_norm.weight", "feature_norm.bias", "feature_norm.offset"}
+    assert set(m.set_feature_head(0).state_dict()) == keys
+    for kind, args in ((ValueError, (5,)), (ValueError, (-1,)), (ValueError, (4, "gelu")), (ValueError, (4, "relu", 1.5)), (ValueError, (4, "relu", 0.1, -1))):
+        with pytest.raises(kind):
+            m.set_feature_head(*args)
+        assert m.feature_norm is None
+    with pytest.raises(NotImplementedError):
+        Generator(hidden_dims=[16, 20], lu_channels=5, scale_factor=1).set_feature_head(4)
+    # configuration: a file without a head is one that the reference reads
+    cfg = Config()
+    cfg.to_yaml(str(tmp_path / "a.yaml"))
+    assert "feature" not in (tmp_path / "a.yaml").read_text()
+    cfg.model.feature_groups = 8
+    cfg.to_yaml(str(tmp_path / "b.yaml"))
+    assert Config.from_yaml(str(tmp_path / "b.yaml")) == cfg
+    # the descriptor's own check
+    from pl_convlstm_gan_amd import _lib
+    d = _lib.RolloutDesc()
+    for k, v in dict(B=1, T=2, H=16, W=16, C1=16, C2=32, L=5, dem_H=16, dem_W=16, lu_H=16, lu_W=16, mid_H=16, mid_W=16, out_H=16, out_W=16).items():
+        setattr(d, k, v)
+    plain = _lib.lib().plc_generator_workspace_bytes(C.byref(d))
+    d.head_groups, d.head_eps = 8, 1e-5
+    assert _lib.lib().plc_generator_workspace_bytes(C.byref(d)) >= plain + 2 * 32 * 256 * 2
+    for k, v in (("head_groups", 5), ("head_groups", -1), ("head_act", 9), ("head_p", 2.0)):
+        old = getattr(d, k)
+        setattr(d, k, v)
+        assert _lib.lib().plc_generator_workspace_bytes(C.byref(d)) == 0, k
+        setattr(d, k, old)
