@@ -277,7 +277,12 @@ static int norm_plan(const plc_norm_desc* d, bool backward, NormArgs* a, NormPla
                 if (need > limit || !(tiles >= (limit == 4 ? 256 : 512) || (limit == 4 && ut / 2 < m0))) continue;
                 a->ut = ut;
                 pl->ku = limit;
-                pl->threads = cdiv(d->HW, 256 / ut) <= 4 ? 256 : 512;
+                pl->threads = 512;
+                for (int n = 64; n < 512; n *= 2)
+                    if (n >= ut && cdiv(d->HW, n / ut) <= 4) {
+                        pl->threads = n;
+                        break;
+                    }
                 break;
             }
     }

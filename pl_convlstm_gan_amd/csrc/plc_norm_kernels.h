@@ -89,12 +89,71 @@ __device__ __forceinline__ NormTid norm_tid(const NormArgs& a, const NormBlock& 
     return t;
 }
 
+// ---- sums over lanes ----------------------------------------------------------------------------------------------
+// Lane shifts inside the vector unit: shuffles go through LDS, at about ten times the latency, and every workgroup needs a few
+// of these before it can do anything else.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float norm_lane_add(float v) {
+    const int moved = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false);
+    return v + __builtin_bit_cast(float, moved);
+}
+// sum of the lanes that agree modulo NU (a power of two up to 16), in every lane
+template <int NU>
+__device__ __forceinline__ float norm_lane_sum(float v) {
+    if (NU <= 8) v = norm_lane_add<0x128, 0xf>(v);      // row_ror:8, 4, 2, 1: rotations within 16 lanes
+    if (NU <= 4) v = norm_lane_add<0x124, 0xf>(v);
+    if (NU <= 2) v = norm_lane_add<0x122, 0xf>(v);
+    if (NU <= 1) v = norm_lane_add<0x121, 0xf>(v);
+    // rows of 16: v_permlane16_swap of a value with itself leaves (rows 0 0 2 2, rows 1 1 3 3), v_permlane32_swap the halves
+    // (the results go through scalars: a bit cast of a vector's element reads element 0)
+    const unsigned x = __builtin_bit_cast(unsigned, v);
+    const auto p = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    const unsigned p0 = p[0], p1 = p[1];
+    v = __builtin_bit_cast(float, p0) + __builtin_bit_cast(float, p1);
+    const unsigned y = __builtin_bit_cast(unsigned, v);
+    const auto q = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+    const unsigned q0 = q[0], q1 = q[1];
+    return __builtin_bit_cast(float, q0) + __builtin_bit_cast(float, q1);
+}
+__device__ __forceinline__ float norm_wave_sum(float v) { return norm_lane_sum<1>(v); }
+
+// Sums over the rows where the lanes of a wave that hold one unit are those that agree modulo nu (NHWC rows of 1, 2, 4, 8 or 16 units;
+// CB8 tiles of one): added across the lanes, then one value per wave.  Two barriers and no more LDS than the result times the
+// number of waves; the general form below has four and moves every value through LDS.
+template <int V, int NV, int NU>
+__device__ __forceinline__ void norm_sum_waves(const float (&v)[NV][V], float* scratch, float* out) {
+    constexpr int nch = NU * V;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float s = norm_lane_sum<NU>(v[k][i]);
+            if (lane < NU) scratch[(wave * NV + k) * nch + lane * V + i] = s;
+        }
+    __syncthreads();
+    for (int c = threadIdx.x; c < NV * nch; c += blockDim.x) {
+        float s = 0.0f;
+        for (int w = 0; w < waves; ++w) s += scratch[w * NV * nch + c];
+        out[c] = s;
+    }
+    __syncthreads();
+}
+
 // ---- sums over the rows of a workgroup --------------------------------------------------------------------------
 // Every thread brings NV values per channel of its unit; out[k * nch + channel of the tile] (LDS) receives their sums over
 // the rows, in a fixed order: a thread per (channel, share of the rows), then one per channel.  Scratch: NV * V * (threads +
 // tile units) floats, padded so that the lanes of a wave read different banks.  Begins and ends with a barrier.
 template <int V, int NV>
-__device__ __forceinline__ void norm_sum_rows(const NormTid& t, int nu, const float (&v)[NV][V], float* scratch, float* out) {
+__device__ __forceinline__ void norm_sum_rows(const NormTid& t, bool px_first, int nu, const float (&v)[NV][V], float* scratch, float* out) {
+    if (nu == 1) return norm_sum_waves<V, NV, 1>(v, scratch, out);
+    if (!px_first) {
+        if (nu == 2) return norm_sum_waves<V, NV, 2>(v, scratch, out);
+        if (nu == 4) return norm_sum_waves<V, NV, 4>(v, scratch, out);
+        if (nu == 8) return norm_sum_waves<V, NV, 8>(v, scratch, out);
+        if (nu == 16) return norm_sum_waves<V, NV, 16>(v, scratch, out);
+    }
     const int nch = nu * V, pitch = blockDim.x + nu;
     __syncthreads();
     if (t.on) {
@@ -143,23 +202,6 @@ __device__ __forceinline__ void norm_sum_rows(const NormTid& t, int nu, const fl
 }
 // floats of LDS for the above: out and scratch
 __host__ __device__ constexpr int norm_lds_floats(int threads, int nu, int V, int NV) { return NV * nu * V + NV * V * (threads + nu); }
-
-// Sum over the 64 lanes, in every lane.  Lane shifts inside the vector unit: shuffles go through LDS, at about ten times
-// the latency, and every workgroup of the second passes starts with a few of these.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ float norm_lane_add(float v) {
-    const int moved = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false);
-    return v + __builtin_bit_cast(float, moved);
-}
-__device__ __forceinline__ float norm_wave_sum(float v) {
-    v = norm_lane_add<0x111, 0xf>(v);      // row_shr:1, 2, 4, 8: lane 15 of each row of 16 has the row's sum
-    v = norm_lane_add<0x112, 0xf>(v);
-    v = norm_lane_add<0x114, 0xf>(v);
-    v = norm_lane_add<0x118, 0xf>(v);
-    v = norm_lane_add<0x142, 0xa>(v);      // row_bcast:15 into rows 1 and 3
-    v = norm_lane_add<0x143, 0xc>(v);      // row_bcast:31 into rows 2 and 3: lane 63 has the sum
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
-}
 
 // ---- activation -------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float norm_sigmoid(float z) {
@@ -359,7 +401,7 @@ __global__ __launch_bounds__(256) void plc_norm_stats_kernel(NormArgs a) {
         v[0][i] = count * d;
         v[1][i] = __builtin_fmaf(count * d, d, m2[i]);
     }
-    norm_sum_rows<V, 2>(t, blk.nu, v, scratch, sums);
+    norm_sum_rows<V, 2>(t, a.px_first, blk.nu, v, scratch, sums);
     // channels -> groups, one wave per group
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6, entries = a.splits * a.parts;
     const int width = a.parts == 1 ? a.cg : nch;
@@ -450,7 +492,7 @@ __device__ __forceinline__ void norm_bwd_reduce(const NormArgs& a, const NormBlo
         float one[1][V];
 #pragma unroll
         for (int i = 0; i < V; ++i) one[0][i] = v[j][i];
-        norm_sum_rows<V, 1>(t, blk.nu, one, scratch, sums + j * nch);
+        norm_sum_rows<V, 1>(t, a.px_first, blk.nu, one, scratch, sums + j * nch);
     }
     float* out = a.part_c + (((long long)blk.n * a.splits + blk.range) * a.C + c0) * 2;
     for (int i = threadIdx.x; i < nch; i += blockDim.x) {
@@ -659,7 +701,7 @@ __global__ __launch_bounds__(512) void plc_norm_fwd_resident_kernel(NormArgs a) 
     }
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
     const float inv = 1.0f / ((float)a.HW * (float)a.cg);
-    norm_sum_rows<V, 1>(t, blk.nu, v, scratch, sums);
+    norm_sum_rows<V, 1>(t, a.px_first, blk.nu, v, scratch, sums);
     for (int g = wave; g < blk.ng; g += waves) {
         float s = 0.0f;
         for (int c = lane; c < a.cg; c += 64) s += sums[g * a.cg + c];
@@ -679,7 +721,7 @@ __global__ __launch_bounds__(512) void plc_norm_fwd_resident_kernel(NormArgs a) 
                 v[0][i] = __builtin_fmaf(d, d, v[0][i]);
             }
     }
-    norm_sum_rows<V, 1>(t, blk.nu, v, scratch, sums);
+    norm_sum_rows<V, 1>(t, a.px_first, blk.nu, v, scratch, sums);
     for (int g = wave; g < blk.ng; g += waves) {
         float s = 0.0f;
         for (int c = lane; c < a.cg; c += 64) s += sums[g * a.cg + c];
