@@ -409,7 +409,8 @@ int plc_dp_unpack_grads(const plc_opt_tensor* t, int n, const float* flat, long 
  * step evaluation), group norm with an activation, dropout.
  *
  * Element types of x, f, y and of the gradients of these: PLC_F32, PLC_BF16, PLC_F16; everything that is summed or
- * carried (states, statistics, gradients of norm weights) is fp32.  Tensors need the alignment of their elements only
+ * carried (states, statistics, gradients of norm weights) is fp32.  Outputs must not overlap inputs except where it
+ * is said.  Tensors need the alignment of their elements only
  * (16-byte aligned ones with strides that are multiples of 16 bytes take the wide accesses).  Empty sizes are
  * allowed and launch nothing, except that norm weight gradients over nothing are set to 0.
  * ------------------------------------------------------------------------------------- */

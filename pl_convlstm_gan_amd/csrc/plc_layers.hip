@@ -49,6 +49,7 @@ extern "C" int plc_dropout(const void* x, const void* residual, void* y, long lo
     if (n == 0) return PLC_OK;
     PLC_REQUIRE(x && y, "dropout: null tensor pointer");
     PLC_REQUIRE((((uintptr_t)x | (uintptr_t)y | (uintptr_t)residual) & (e - 1)) == 0, "dropout: misaligned tensor pointer");
+    PLC_REQUIRE((((uintptr_t)offset_ptr | (uintptr_t)used_offset) & 7) == 0, "dropout: misaligned offset pointer");
     DropoutArgs a;
     a.n = n;
     a.x = x;
@@ -231,6 +232,8 @@ static int norm_plan(const plc_norm_desc* d, bool backward, NormArgs* a, NormPla
     PLC_REQUIRE(d->layout == PLC_NHWC || e == 2, "group norm: the CB8 layout holds 16-bit elements");
     PLC_REQUIRE(d->eps >= 0.0f, "group norm: negative eps");
     PLC_REQUIRE(d->p >= 0.0 && d->p <= 1.0, "group norm: p = %g is not a probability", d->p);
+    PLC_REQUIRE((((uintptr_t)d->offset_ptr | (uintptr_t)d->used_offset) & 7) == 0, "group norm: misaligned offset pointer");
+    if (d->HW > 1 << 30) return plc_fail(PLC_EUNSUPPORTED, "group norm: %d pixels are more than 2^30", d->HW);
     const void* types[] = {d->x, d->y, d->dy, d->dx};
     for (const void* p : types) PLC_REQUIRE(((uintptr_t)p & (e - 1)) == 0, "group norm: misaligned tensor pointer");
     memset(a, 0, sizeof(*a));

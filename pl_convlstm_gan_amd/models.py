@@ -138,6 +138,11 @@ class Generator(nn.Module):
         self._ws = {}
         self._tabs = {}
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if "feature_norm" not in self.__dict__ and "feature_norm" not in self._modules:      # (pickled before the head existed)
+            self.feature_norm = None
+
     def set_feature_head(self, num_groups, act="silu", p=0.0, seed=0):
         """Adds group norm + activation (+ dropout of probability ``p`` in training mode) on the recurrence's features, in front
         of the upsample blocks.  Not a constructor argument: the reference has none, and without this call the model, its

@@ -162,6 +162,68 @@ def test_step_by_step_is_the_scan(layers, gpu, dtype):
         assert torch.equal(state, h)
 
 
+@pytest.mark.parametrize("T", [1, 30, 700])
+def test_scan_state_in_place(layers, gpu, T):
+    """The last state may overwrite the first, also where the sequence is worked on in segments."""
+    from pl_convlstm_gan_amd import ops
+    x, f, h0 = rand((2, T, 6), 1, torch.float32, gpu), rand((2, T, 6), 2, torch.float32, gpu), rand((2, 6), 3, torch.float32, gpu)
+    y, h, _ = ops.gated_scan_forward(x, f, h0)
+    state = h0.clone()
+    y2, h2, _ = ops.gated_scan_forward(x, f, state, h_last=state)
+    assert h2.data_ptr() == state.data_ptr() and torch.equal(y, y2) and torch.equal(h, state)
+
+
+def test_explicit_passes_are_autograds(layers, gpu):
+    """ops.*_forward / *_backward, the passes without autograd, give what autograd gives, bit for bit."""
+    from pl_convlstm_gan_amd import ops
+    x, f, h0 = rand((2, 50, 6), 1, torch.bfloat16, gpu), rand((2, 50, 6), 2, torch.bfloat16, gpu), rand((2, 6), 3, torch.float32, gpu)
+    dy, dh = rand((2, 50, 6), 4, torch.bfloat16, gpu), rand((2, 6), 5, torch.float32, gpu)
+    n = torch.tensor([50, 11], dtype=torch.int32, device=gpu)
+    _, _, states = ops.gated_scan_forward(x, f, h0, n, True, save_states=True)
+    a = ops.gated_scan_backward(x, f, h0, n, True, states, dy, dh)
+    leaves = [t.clone().requires_grad_() for t in (x, f, h0)]
+    b = torch.autograd.grad(layers.gated_linear_scan(*leaves, lengths=n), leaves, (dy, dh))
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    x, w = rand((2, 12, 9, 7), 6, torch.float32, gpu), rand((12,), 7, torch.float32, gpu)
+    dy = rand((2, 12, 9, 7), 8, torch.float32, gpu)
+    y, stats = ops.group_norm_forward(x, 3, w, None, 1e-5, "silu", 0.2, 5, 6)
+    a = ops.group_norm_backward(x, 3, w, None, 1e-5, "silu", 0.2, 5, 6, stats, dy)
+    leaves = [t.clone().requires_grad_() for t in (x, w)]
+    z = layers.group_norm_act(leaves[0], 3, leaves[1], None, act="silu", p=0.2, seed=5, offset=6)
+    b = torch.autograd.grad(z, leaves, dy)
+    assert torch.equal(y, z) and torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and a[2] is None
+    with pytest.raises(ValueError, match="states"):
+        ops.gated_scan_backward(rand((2, 50, 6), 1, torch.bfloat16, gpu), f[:, :50], h0, n, True, None, rand((2, 50, 6), 4, torch.bfloat16, gpu), dh)
+
+
+def test_changed_inputs_are_refused_in_the_backward_pass(layers, gpu):
+    x, f = (rand((1, 20, 8), k, torch.float32, gpu).requires_grad_() for k in (1, 2))
+    a = x * 1
+    y, _ = layers.gated_linear_scan(a, f)
+    a.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_two_threads_at_once(layers, gpu):
+    """Calls from two host threads, each on its own stream: the results of the calls alone."""
+    import threading
+    leaves, _ = block_inputs(gpu, torch.bfloat16)
+    leaves = [t.detach() for t in leaves]
+    want = [block(layers, *leaves, o)[0] for o in (1, 2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i].append(block(layers, *leaves, i + 1)[0])
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads], [t.join() for t in threads]
+    assert all(len(g) == 20 and all(torch.equal(o, w) for o in g) for g, w in zip(got, want))
+
+
 def test_scan_pieces_carry_the_state(layers, gpu):
     """A sequence in two pieces, the state carried in fp32: the same as in one, values and gradients."""
     x, f = rand((2, 90, 12), 1, torch.bfloat16, gpu).requires_grad_(), rand((2, 90, 12), 2, torch.bfloat16, gpu).requires_grad_()
@@ -499,3 +561,32 @@ def test_refusals(layers, gpu):
         with pytest.raises(kind):
             call()
             pytest.fail(f"case {k} was not refused")
+
+
+def test_offsets_beyond_32_bits(layers, gpu):
+    """More than 2^31 elements: the ends of the tensors against the same calls on their slices."""
+    n = (1 << 31) + 1003
+    x = torch.ones(n, dtype=torch.bfloat16, device=gpu)
+    y = layers.counter_dropout(x, 0.5, 77, 5)
+    tail = n - 4096 - n % 8
+    j = R.np.arange(tail // 8, (n + 7) // 8, dtype=R.np.uint64)
+    w = R.philox([j & R.np.uint64(0xFFFFFFFF), j >> R.np.uint64(32), R.np.full_like(j, 5), R.np.full_like(j, 0)], (77, 0))
+    u16 = R.np.stack([w[i // 2] >> R.np.uint64(16 * (i % 2)) & R.np.uint64(0xFFFF) for i in range(8)], 1).reshape(-1)[:n - tail]
+    assert torch.equal(y[tail:] != 0, torch.from_numpy(u16 >= 32768).to(gpu))
+    del x, y
+    D = (1 << 31) + 24
+    x = torch.full((1, 2, D), 0.5, dtype=torch.bfloat16, device=gpu)
+    f = torch.zeros(1, 2, D, dtype=torch.bfloat16, device=gpu)
+    x[0, :, -100:], f[0, :, -100:] = rand((2, 100), 1, torch.bfloat16, gpu), rand((2, 100), 2, torch.bfloat16, gpu)
+    y, h = layers.gated_linear_scan(x, f)
+    a, b = layers.gated_linear_scan(x[:, :, -100:].contiguous(), f[:, :, -100:].contiguous())
+    assert torch.equal(y[:, :, -100:], a) and torch.equal(h[:, -100:], b) and float(h[0, 0]) == 0.375
+    del x, f, y, h
+    torch.cuda.empty_cache()
+    shape = (3, 4700, 4800, 32)
+    x = torch.empty(shape, dtype=torch.bfloat16, device=gpu).normal_().permute(0, 3, 1, 2)
+    y = layers.group_norm_act(x, 4, act="relu")
+    assert torch.equal(y[2:], layers.group_norm_act(x[2:], 4, act="relu"))
+    z = layers.group_norm_act(x, 4, act="relu", p=0.5, seed=1)[2].permute(1, 2, 0).reshape(-1)
+    keep = layers.counter_dropout(torch.ones(3 * 4700 * 4800 * 32, dtype=torch.bfloat16, device=gpu), 0.5, 1)[-z.numel():] != 0
+    assert float(z[~keep].abs().max()) == 0 and torch.equal(z[keep], (y[2].permute(1, 2, 0).reshape(-1)[keep].float() * 2).to(torch.bfloat16))

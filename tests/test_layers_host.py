@@ -59,6 +59,12 @@ def test_scan_abi_refusals():
                      (dict(dy=4098), "misaligned"), (dict(dh_last=4099), "misaligned")):
         refused(L.plc_gated_scan_bwd(C.byref(scan_desc(**kw)), None), -1, text)
     refused(L.plc_gated_scan_fwd(C.byref(scan_desc(B=1 << 30, D=1 << 20)), None), -2, "one launch")
+    refused(L.plc_gated_scan_fwd(C.byref(scan_desc(T=(1 << 30) + 1)), None), -2, "2^30")
+    long = scan_desc(T=5000)                     # (few channels, many steps: works in segments and needs room for their sums)
+    assert L.plc_gated_scan_workspace_bytes(C.byref(long), 0) > 0 and L.plc_gated_scan_workspace_bytes(C.byref(scan_desc(T=8)), 0) == 0
+    refused(L.plc_gated_scan_fwd(C.byref(long), None), -3, "workspace")
+    refused(L.plc_gated_scan_fwd(C.byref(scan_desc(T=5000, workspace=4096, workspace_bytes=16)), None), -3, "workspace")
+    refused(L.plc_gated_scan_bwd(C.byref(scan_desc(T=5000, workspace=4100, workspace_bytes=1 << 30)), None), -1, "16-byte")
     # nothing to do is no error
     assert L.plc_gated_scan_fwd(C.byref(scan_desc(B=0, x=None, f=None, y=None)), None) == 0
     assert L.plc_gated_scan_states_bytes(2, 8, 8) == 0 and L.plc_gated_scan_states_bytes(2, 33, 8) == 2 * 4 * 8 * 4
@@ -72,11 +78,13 @@ def test_norm_abi_refusals():
     for kw, text in ((dict(dtype=3), "element type"), (dict(N=-1), "bad size"), (dict(C=0), "bad size"), (dict(G=3), "do not divide"), (dict(G=0), "do not divide"),
                      (dict(act=3), "activation"), (dict(layout=2), "layout"), (dict(layout=1, C=12), "whole blocks"), (dict(layout=1, x=4098), "16-byte"),
                      (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(p=2.0), "probability"), (dict(p=float("nan")), "probability"),
-                     (dict(x=4097), "misaligned"), (dict(weight=4098), "misaligned"), (dict(x=None), "null tensor"), (dict(y=None), "null tensor"),
+                     (dict(x=4097), "misaligned"), (dict(weight=4098), "misaligned"), (dict(offset_ptr=4100), "misaligned"), (dict(used_offset=4100), "misaligned"), (dict(x=None), "null tensor"), (dict(y=None), "null tensor"),
                      (dict(stats=None), "null tensor"), (dict(workspace=None), "null workspace")):
         refused(L.plc_group_norm_fwd(C.byref(norm_desc(**kw)), None), -1, text)
     refused(L.plc_group_norm_bwd(C.byref(norm_desc(dy=None)), None), -1, "null tensor")
     refused(L.plc_group_norm_fwd(C.byref(norm_desc(workspace_bytes=1)), None), -3, "workspace")
+    refused(L.plc_group_norm_fwd(C.byref(norm_desc(HW=(1 << 30) + 1)), None), -2, "2^30")
+    refused(L.plc_group_norm_fwd(C.byref(norm_desc(layout=1, dtype=0)), None), -1, "16-bit")
     refused(L.plc_group_norm_fwd(C.byref(norm_desc(N=(1 << 31) - 1, workspace_bytes=1 << 50)), None), -2, "one launch")
     need = L.plc_group_norm_workspace_bytes(C.byref(norm_desc()), 0)
     assert need > 0 and L.plc_group_norm_workspace_bytes(C.byref(norm_desc(G=5)), 1) == 0
@@ -91,6 +99,8 @@ def test_dropout_abi_refusals():
                      (dict(p=float("nan")), "probability"), (dict(x=None), "null"), (dict(y=None), "null"), (dict(x=4098), "misaligned"), (dict(r=4097), "misaligned")):
         refused(call(**kw), -1, text)
     refused(call(n=1 << 45), -2, "one launch")
+    refused(L.plc_dropout(4096, None, 8192, 100, 0, 0.5, 1, 2, 4100, None, None), -1, "misaligned offset")
+    refused(L.plc_dropout(4096, None, 8192, 100, 0, 0.5, 1, 2, None, 4100, None), -1, "misaligned offset")
     assert call(n=0, x=None, y=None) == 0
 
 
@@ -162,6 +172,13 @@ def test_feature_head_interface(tmp_path):
         assert m.feature_norm is None
     with pytest.raises(NotImplementedError):
         Generator(hidden_dims=[16, 20], lu_channels=5, scale_factor=1).set_feature_head(4)
+    # a model pickled before the head existed has none
+    state = dict(m.__dict__)
+    state.pop("feature_norm", None)
+    state["_modules"] = {k: v for k, v in m._modules.items() if k != "feature_norm"}
+    old = Generator.__new__(Generator)
+    old.__setstate__(state)
+    assert old.feature_norm is None
     # configuration: a file without a head is one that the reference reads
     cfg = Config()
     cfg.to_yaml(str(tmp_path / "a.yaml"))
