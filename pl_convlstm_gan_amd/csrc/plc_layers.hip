@@ -266,8 +266,8 @@ static int norm_plan(const plc_norm_desc* d, bool backward, NormArgs* a, NormPla
     a->ps = a->px_first ? 8 : d->C;
     a->splits = 1;
     a->px_split = d->HW;
-    // Resident form, where the chip is full of tiles of at most four units a thread (rows of up to 128 bytes as long as they
-    // leave 256 tiles), or of larger ones that are many.
+    // Resident form: tiles of at most four units a thread (workgroups of up to 1024, rows of up to 128 bytes as long as that
+    // leaves 256 tiles), or larger ones that are many (512 threads, whose registers hold them).
     const int ku_max = backward ? 8 : 16;
     if (a->parts == 1 && m0 <= 64 && d->HW > 0 && (long long)d->HW * m0 <= 512ll * ku_max) {
         int widest = m0;
@@ -275,13 +275,13 @@ static int norm_plan(const plc_norm_desc* d, bool backward, NormArgs* a, NormPla
             while (a->U % (widest * 2) == 0 && widest * v * e < 128) widest *= 2;
         for (int limit = 4; limit <= ku_max && !pl->ku; limit = limit == 4 ? ku_max : 2 * ku_max)
             for (int ut = widest; ut >= m0; ut /= 2) {
-                const int need = cdiv(d->HW, 512 / ut);
+                const int most = limit == 4 ? 1024 : 512, need = cdiv(d->HW, most / ut);
                 const long long tiles = (long long)d->N * (a->U / ut);
                 if (need > limit || !(tiles >= (limit == 4 ? 256 : 512) || (limit == 4 && ut / 2 < m0))) continue;
                 a->ut = ut;
                 pl->ku = limit;
-                pl->threads = 512;
-                for (int n = 64; n < 512; n *= 2)
+                pl->threads = most;
+                for (int n = 64; n < most; n *= 2)
                     if (n >= ut && cdiv(d->HW, n / ut) <= 4) {
                         pl->threads = n;
                         break;

@@ -117,6 +117,16 @@ __device__ __forceinline__ float norm_lane_sum(float v) {
 }
 __device__ __forceinline__ float norm_wave_sum(float v) { return norm_lane_sum<1>(v); }
 
+// sum over a workgroup of up to 16 waves, in every thread; scratch: 16 floats of LDS that nothing else uses; one barrier
+__device__ __forceinline__ float norm_block_sum(float v, float* scratch) {
+    v = norm_wave_sum(v);
+    if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float s = 0.0f;
+    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) s += scratch[w];
+    return s;
+}
+
 // Sums over the rows where the lanes of a wave that hold one unit are those that agree modulo nu (NHWC rows of 1, 2, 4, 8 or 16 units;
 // CB8 tiles of one): added across the lanes, then one value per wave.  Two barriers and no more LDS than the result times the
 // number of waves; the general form below has four and moves every value through LDS.
@@ -675,7 +685,7 @@ __device__ __forceinline__ unsigned norm_xcd_order(unsigned i, unsigned n) {
 }
 
 template <class T, int V, int FORM, int KU>
-__global__ __launch_bounds__(512) void plc_norm_fwd_resident_kernel(NormArgs a) {
+__global__ __launch_bounds__(KU == 4 ? 1024 : 512) void plc_norm_fwd_resident_kernel(NormArgs a) {
     extern __shared__ __align__(16) float lds[];
     const NormBlock blk = norm_block<V>(a, norm_xcd_order(blockIdx.x, gridDim.x), 1);
     const NormTid t = norm_tid(a, blk);
@@ -691,49 +701,75 @@ __global__ __launch_bounds__(512) void plc_norm_fwd_resident_kernel(NormArgs a) 
 #pragma unroll
     for (int j = 0; j < KU; ++j)
         if (t.on && t.r + j * t.rows < a.HW) raw[j] = plc_load<T, V>(x + (long long)(t.r + j * t.rows) * a.ps);
-    float v[1][V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        v[0][i] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < KU; ++j)
-            if (t.on && t.r + j * t.rows < a.HW) v[0][i] += raw[j].get(i);
-    }
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
     const float inv = 1.0f / ((float)a.HW * (float)a.cg);
-    norm_sum_rows<V, 1>(t, a.px_first, blk.nu, v, scratch, sums);
-    for (int g = wave; g < blk.ng; g += waves) {
-        float s = 0.0f;
-        for (int c = lane; c < a.cg; c += 64) s += sums[g * a.cg + c];
-        s = norm_wave_sum(s);
-        if (lane == 0) st[2 * g] = s * inv;
-    }
-    __syncthreads();
-    float mean[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        mean[i] = t.on ? st[2 * ((u * V + i) / a.cg - blk.g0)] : 0.0f;
-        v[0][i] = 0.0f;
+    float* const stats = a.stats + ((long long)blk.n * a.G + blk.g0) * 2;
+    if (blk.ng == 1) {
+        // the tile is one group: one number per thread, not one per channel
+        float s = 0.0f, q = 0.0f;
 #pragma unroll
         for (int j = 0; j < KU; ++j)
-            if (t.on && t.r + j * t.rows < a.HW) {
-                const float d = raw[j].get(i) - mean[i];
-                v[0][i] = __builtin_fmaf(d, d, v[0][i]);
-            }
-    }
-    norm_sum_rows<V, 1>(t, a.px_first, blk.nu, v, scratch, sums);
-    for (int g = wave; g < blk.ng; g += waves) {
-        float s = 0.0f;
-        for (int c = lane; c < a.cg; c += 64) s += sums[g * a.cg + c];
-        s = norm_wave_sum(s);
-        if (lane == 0) {
-            const float r = 1.0f / sqrtf(s * inv + a.eps);
-            st[2 * g + 1] = r;
-            a.stats[((long long)blk.n * a.G + blk.g0 + g) * 2] = st[2 * g];
-            a.stats[((long long)blk.n * a.G + blk.g0 + g) * 2 + 1] = r;
+            if (t.on && t.r + j * t.rows < a.HW)
+#pragma unroll
+                for (int i = 0; i < V; ++i) s += raw[j].get(i);
+        const float m = norm_block_sum(s, scratch) * inv;
+#pragma unroll
+        for (int j = 0; j < KU; ++j)
+            if (t.on && t.r + j * t.rows < a.HW)
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float d = raw[j].get(i) - m;
+                    q = __builtin_fmaf(d, d, q);
+                }
+        const float r = 1.0f / sqrtf(norm_block_sum(q, scratch + 16) * inv + a.eps);
+        if (threadIdx.x == 0) {
+            st[0] = stats[0] = m;
+            st[1] = stats[1] = r;
         }
+        __syncthreads();
+    } else {
+        float v[1][V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            v[0][i] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < KU; ++j)
+                if (t.on && t.r + j * t.rows < a.HW) v[0][i] += raw[j].get(i);
+        }
+        norm_sum_rows<V, 1>(t, a.px_first, blk.nu, v, scratch, sums);
+        for (int g = wave; g < blk.ng; g += waves) {
+            float s = 0.0f;
+            for (int c = lane; c < a.cg; c += 64) s += sums[g * a.cg + c];
+            s = norm_wave_sum(s);
+            if (lane == 0) st[2 * g] = s * inv;
+        }
+        __syncthreads();
+        float mean[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            mean[i] = t.on ? st[2 * ((u * V + i) / a.cg - blk.g0)] : 0.0f;
+            v[0][i] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < KU; ++j)
+                if (t.on && t.r + j * t.rows < a.HW) {
+                    const float d = raw[j].get(i) - mean[i];
+                    v[0][i] = __builtin_fmaf(d, d, v[0][i]);
+                }
+        }
+        norm_sum_rows<V, 1>(t, a.px_first, blk.nu, v, scratch, sums);
+        for (int g = wave; g < blk.ng; g += waves) {
+            float s = 0.0f;
+            for (int c = lane; c < a.cg; c += 64) s += sums[g * a.cg + c];
+            s = norm_wave_sum(s);
+            if (lane == 0) {
+                const float r = 1.0f / sqrtf(s * inv + a.eps);
+                st[2 * g + 1] = r;
+                stats[2 * g] = st[2 * g];
+                stats[2 * g + 1] = r;
+            }
+        }
+        __syncthreads();
     }
-    __syncthreads();
     if (!t.on) return;
     NormUnit<V> k;
     norm_unit<V>(a, blk, t.u, st, k);
@@ -746,7 +782,7 @@ __global__ __launch_bounds__(512) void plc_norm_fwd_resident_kernel(NormArgs a) 
 }
 
 template <class T, int V, int FORM, int KU>
-__global__ __launch_bounds__(512) void plc_norm_bwd_resident_kernel(NormArgs a) {
+__global__ __launch_bounds__(KU == 4 ? 1024 : 512) void plc_norm_bwd_resident_kernel(NormArgs a) {
     extern __shared__ __align__(16) float lds[];
     const NormBlock blk = norm_block<V>(a, norm_xcd_order(blockIdx.x, gridDim.x), 1);
     const NormTid t = norm_tid(a, blk);
