@@ -238,7 +238,6 @@ static int cu_count() {
     }
     return cached[dev];
 }
-int plc_cu_count() { return cu_count(); }
 
 // Raises a kernel's dynamic-LDS limit once per (kernel, device) instead of on every launch; `done` is
 // the per-instantiation flag array of the caller.

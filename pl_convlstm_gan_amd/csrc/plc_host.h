@@ -11,7 +11,6 @@
 // stores the message plc_last_error() returns on this thread and gives `code` back
 PLC_HIDDEN int plc_fail(int code, const char* fmt, ...);
 // number of CUs of the current device (looked up once per device)
-PLC_HIDDEN int plc_cu_count();
 
 #define PLC_HIP(expr)                                                                         \
     do {                                                                                      \

@@ -114,12 +114,25 @@ static int scan_check(const plc_scan_desc* d, bool backward, ScanArgs* a, int* v
 }
 
 // How a call runs: channels per lane, and segments of time (1: one lane walks the whole sequence).
-static void scan_plan(ScanArgs* a, int vmax, bool backward, int* v) {
+//
+// One pass costs about 0.11 us a step (a block of SCAN_K steps is one trip to memory) until the rows fill the memory; the
+// split form costs three launches, 8 us, and reads its inputs twice.  So time is split for long sequences of narrow rows.
+// Forward/backward in us, split against one pass, rows of n = B x D numbers (4 samples):
+//   n = 512, bf16:    T = 64   8.1/8.4 against  6.6/9.3     T = 96   8.1/8.3 against  8.8/12.9    T = 1024   9.2/9.4 against  73/140
+//   n = 16000, fp32:  T = 96  14.3/15.7 against 13.2/16.8   T = 128 15.0/16.5 against 16.8/21.2   T = 1024  71/104  against 179/228
+//   n = 80000, bf16:  T = 128 28.8/36.7 against 20.2/32.4   T = 256 49.1/69.4 against 55.9/73.1   T = 1024 197/272  against 221/288
+//   n = 80000, fp32:  T = 128 42.2/61.6 against 33.2/45.5   T = 256 92/128    against 64.5/94.5   (one pass at every length)
+//
+// Without the split, lanes take fewer channels until 1024 waves share the rows: more loads are in flight.  With 16 x 40000
+// bf16 of 4 samples four channels per lane cost 6.9/9.0 us, two 6.2/8.3; 24 x 8192 fp32 of 8 samples 8.6/13.7 with four, 6.4/8.3 with one.
+// Eight channels (16 bytes of a 16-bit type) pay forward once 4096 waves are left; backward they cost registers, and with
+// them the waves that hide the loads (10 x 2097152 bf16 of 4 samples: 250 us against 190).
+static void scan_plan(ScanArgs* a, int e, int vmax, bool backward, int* v) {
     const long long n = (long long)a->B * a->D;
     *v = vmax < 4 ? vmax : 4;
     a->nseg = 1;
     a->seg = a->T;
-    if (n / *v / 64 < 512 && a->T >= 4 * SCAN_K) {
+    if (n * e <= 160 << 10 && a->T >= 80 + n * e / 1024) {
         *v = vmax >= 2 && n >= 1024 ? 2 : 1;
         const long long most = a->T >= 1 << 18 ? 64 * 4 * SCAN_RUN : 64 * SCAN_RUN;
         long long want = 4096 * 64ll / (n / *v);
@@ -142,8 +155,8 @@ static void scan_carry_runs(const ScanArgs& a, hipStream_t st) {
 }
 template <bool BACKWARD>
 static void scan_carry(const ScanArgs& a, hipStream_t st) {
-    if (a.nseg <= SCAN_RUN) scan_carry_runs<BACKWARD, 1>(a, st);
-    else if (a.nseg <= 4 * SCAN_RUN) scan_carry_runs<BACKWARD, 4>(a, st);
+    if (a.nseg <= 4) scan_carry_runs<BACKWARD, 1>(a, st);
+    else if (a.nseg <= 32) scan_carry_runs<BACKWARD, 4>(a, st);
     else if (a.nseg <= 16 * SCAN_RUN) scan_carry_runs<BACKWARD, 16>(a, st);
     else scan_carry_runs<BACKWARD, 64>(a, st);
 }
@@ -173,7 +186,7 @@ extern "C" size_t plc_gated_scan_workspace_bytes(const plc_scan_desc* d, int bac
     ScanArgs a;
     int v = 1;
     if (scan_check(d, backward != 0, &a, &v) || a.B == 0 || a.D == 0) return 0;
-    scan_plan(&a, v, backward != 0, &v);
+    scan_plan(&a, dtype_size(d->dtype), v, backward != 0, &v);
     return scan_workspace(a);
 }
 
@@ -197,7 +210,7 @@ static int scan_run(const plc_scan_desc* d, bool backward, void* stream) {
     int v = 1;
     const int rc = scan_check(d, backward, &a, &v);
     if (rc || a.B == 0 || a.D == 0) return rc;
-    scan_plan(&a, v, backward, &v);
+    scan_plan(&a, dtype_size(d->dtype), v, backward, &v);
     const size_t need = scan_workspace(a);
     if (need) {
         if (!d->workspace || d->workspace_bytes < need)
@@ -266,9 +279,18 @@ static int norm_plan(const plc_norm_desc* d, bool backward, NormArgs* a, NormPla
     a->ps = a->px_first ? 8 : d->C;
     a->splits = 1;
     a->px_split = d->HW;
-    // Resident form: tiles of at most four units a thread (workgroups of up to 1024, rows of up to 128 bytes as long as that
-    // leaves 256 tiles), or larger ones that are many (512 threads, whose registers hold them).
+    // Resident form (one launch, x read once).  A thread keeps up to four units; or, forward 9 .. 16 and backward 5 .. 8, with
+    // 512 threads, where a workgroup per CU (backward two) is left.  Rows as wide as 128 bytes while enough tiles are left.
+    // Forward/backward in us against the split form (32 channels in 8 groups, bf16, unless said otherwise):
+    //   5 x 15 x 12, fp32          3.9/7.7 against  9.3/10.4      8 x 512 channels in 32 groups, 32 x 32   8.9/17.0 against 23.6/25.6
+    //   128 x 32 x 64             16.9/23.7 against 18.5/24.6      32 x 512 channels in 32 groups, 32 x 32 27.8/44 against 33.3/52.5
+    //   512 x 40 x 40, 1 group    23.5/57.7 against 34.4/58.0
+    // A tensor beyond the caches (20 MB) is another matter.  There the workgroups' loads, sums and stores have to overlap:
+    // workgroups of more than 256 threads with four units each do not (512 x 8 channels x 64 x 64: 30.3/47.6 against 23.6/37.5),
+    // and rows of less than 64 bytes that are part of longer ones move lines more than once (512 x 30 x 24, fp32, 16-byte rows:
+    // 27.9/59.5 against 29.2/46.9).
     const int ku_max = backward ? 8 : 16;
+    const bool large = (double)a->N * (double)a->img * e > 20e6;
     if (a->parts == 1 && m0 <= 64 && d->HW > 0 && (long long)d->HW * m0 <= 512ll * ku_max) {
         int widest = m0;
         if (!a->px_first)
@@ -277,7 +299,14 @@ static int norm_plan(const plc_norm_desc* d, bool backward, NormArgs* a, NormPla
             for (int ut = widest; ut >= m0; ut /= 2) {
                 const int most = limit == 4 ? 1024 : 512, need = cdiv(d->HW, most / ut);
                 const long long tiles = (long long)d->N * (a->U / ut);
-                if (need > limit || !(tiles >= (limit == 4 ? 256 : 512) || (limit == 4 && ut / 2 < m0))) continue;
+                const bool lines = ut * v * e >= 64;
+                if (need > limit) continue;
+                if (limit == 4) {
+                    if (tiles < 256 && ut / 2 >= m0) continue;
+                    if (large && !((lines || ut == a->U || a->px_first) && cdiv(d->HW, 256 / ut) <= 4)) continue;
+                } else if (tiles < (backward ? 512 : 256) || need <= ku_max / 2 || (backward && !lines)) {
+                    continue;
+                }
                 a->ut = ut;
                 pl->ku = limit;
                 pl->threads = most;
@@ -296,7 +325,8 @@ static int norm_plan(const plc_norm_desc* d, bool backward, NormArgs* a, NormPla
         pl->threads = 256;
         const int rows = 256 / a->ut, p = backward ? NORM_PB : NORM_P;
         a->tiles = a->parts > 1 ? a->G * a->parts : cdiv(a->U, a->ut);
-        // pixel ranges: enough workgroups for the chip, two rounds of loads each at least, at most 64 per sample
+        // Pixel ranges: two rounds of loads each at least, at most 256 per sample, and enough for 4096 workgroups: with 40 samples
+        // of 256 x 256 x 32 in bf16 1024 of them cost 120/203 us, 2048 110/186, 4096 105/175, 8192 105/171; smaller calls do not differ.
         const long long per = (long long)d->N * a->tiles, want = per > 0 ? (4096 + per - 1) / per : 1;
         const long long most = d->HW > 0 ? (d->HW + 2 * p * rows - 1) / (2 * p * rows) : 1;
         long long s = want < most ? want : most;

@@ -79,17 +79,6 @@ __device__ __forceinline__ float plc_exp_neg(float x) {
     return t < -126.0f ? e : __builtin_fmaf(e * 0.693147180559945309f, lo, e);
 }
 
-// s = sigmoid(x) and q = 1 - s = sigmoid(-x), each to a few units in ITS last place (q is not formed by
-// subtraction: a gate near 1 would lose it).  Infinities give 0 and 1, NaN stays NaN.
-__device__ __forceinline__ void plc_sigmoid_pair(float x, float& s, float& q) {
-    const float e = plc_exp_neg(-__builtin_fabsf(x));
-    const float r = __builtin_amdgcn_rcpf(1.0f + e);
-    const float er = e * r;
-    const bool pos = x >= 0.0f;
-    s = pos ? r : er;
-    q = pos ? er : r;
-}
-
 // Philox4x32-10 (Salmon, Moraes, Dror, Shaw: Parallel random numbers: as easy as 1, 2, 3; SC 2011): 128 random bits
 // that depend on the counter and the key alone.
 __device__ __forceinline__ uint4 plc_philox(uint64_t lo, uint64_t hi, uint64_t key) {

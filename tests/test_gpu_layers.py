@@ -225,17 +225,28 @@ def test_two_threads_at_once(layers, gpu):
 
 
 def test_scan_pieces_carry_the_state(layers, gpu):
-    """A sequence in two pieces, the state carried in fp32: the same as in one, values and gradients."""
+    """A sequence in two pieces, the state carried in fp32: as in one, values and gradients.  The bits need not agree: the
+    sequence in one call may be computed as segments whose maps h -> A h + S are joined, the pieces step by step.  Either
+    is within e + r of the 64-bit value v (e the recurrence's bound over all 90 steps, r half a step of the type), so by the
+    triangle inequality they are within 2 (e + r) of one another; both bounds are checked as |one - v|, |two - v| <= e + r."""
     x, f = rand((2, 90, 12), 1, torch.bfloat16, gpu).requires_grad_(), rand((2, 90, 12), 2, torch.bfloat16, gpu).requires_grad_()
     y, h = layers.gated_linear_scan(x, f)
     a, ha = layers.gated_linear_scan(x[:, :48], f[:, :48])
     b, hb = layers.gated_linear_scan(x[:, 48:], f[:, 48:], ha)
-    assert torch.equal(torch.cat([a, b], 1), y) and torch.equal(hb, h)
     dy = rand((2, 90, 12), 3, torch.bfloat16, gpu)
     one = torch.autograd.grad(y, (x, f), dy)
     two = torch.autograd.grad((a, b), (x, f), (dy[:, :48], dy[:, 48:]))
-    for p, q in zip(one, two):
-        assert torch.equal(p, q)
+    val, err = R.scan(x, f, None, None, True, dy)
+    for k, p, q in zip(("y", "h_last", "dx", "df"), (y, h) + one, (torch.cat([a, b], 1), hb) + two):
+        R.check(p, val[k], err[k], k + " in one")
+        R.check(q, val[k], err[k], k + " in two pieces")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,D", [(1, 79, 6), (1, 80, 6), (2, 96, 1024), (3, 127, 2048), (3, 250, 2048), (2, 129, 1030), (1, 2100, 40), (1, 9000, 16), (2, 300, 20482)])
+def test_scan_around_the_split(layers, gpu, dtype, B, T, D):
+    """Lengths and widths on both sides of every choice between one pass and segments, and of the carry's run lengths."""
+    scan_case(layers, gpu, (B, T, D), dtype, True, [T - 3, T // 2, T][:B])
 
 
 def test_scan_gradient_against_differences(layers, gpu):
@@ -348,6 +359,13 @@ def test_norm_types_and_activations(layers, gpu, p, act, dtype):
 def test_norm_shapes(layers, gpu, shape, groups, dtype):
     norm_case(layers, gpu, shape, groups, dtype)
     norm_case(layers, gpu, shape, groups, dtype, "relu", 0.2, seed=9)
+
+
+@pytest.mark.parametrize("shape,groups,dtype", [((256, 32, 30, 24), 8, torch.float32), ((256, 32, 41, 40), 1, torch.bfloat16), ((640, 32, 23, 23), 8, torch.float16),
+                                                ((530, 24, 30, 31), 3, torch.bfloat16), ((40, 512, 23, 24), 32, torch.float16)])
+def test_norm_beyond_the_caches(layers, gpu, shape, groups, dtype):
+    """More than 20 MB in many small samples, where the choice between the forms is another one."""
+    norm_case(layers, gpu, shape, groups, dtype, "silu")
 
 
 def test_norm_without_affine_and_far_mean(layers, gpu):
