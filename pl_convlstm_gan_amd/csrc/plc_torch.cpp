@@ -83,6 +83,10 @@ void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device
 template <class T = void>
 T* ptr(const Tensor& t) { return t.defined() ? reinterpret_cast<T*>(t.data_ptr()) : nullptr; }
 Tensor get(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+// A kernel has written into a caller's tensor: a backward pass that kept it has to notice.
+void written(const Tensor& t) {
+    if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 Tensor workspace(size_t bytes, const Tensor& x) {
     return bytes ? at::empty({(int64_t)bytes}, x.options().dtype(at::kByte)) : Tensor();
 }
@@ -182,6 +186,7 @@ std::tuple<Tensor, Tensor, Tensor> scan_forward(const Tensor& x, const Tensor& f
     s.d.workspace = ptr(ws);
     s.d.workspace_bytes = n;
     check_rc(lib.scan_fwd(&s.d, stream_of(x)), "plc_gated_scan_fwd");
+    written(into);
     return {y, h, states};
 }
 
@@ -304,6 +309,7 @@ Tensor dropout_forward(const Tensor& x_, double p, uint64_t seed, uint64_t offse
     Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
     check_rc(lib.dropout(ptr(x), ptr(r), ptr(y), x.numel(), dtype, p, seed, offset, ptr<long long>(offset_t), ptr<long long>(used), stream_of(x)),
              "plc_dropout");
+    written(used);
     return y;
 }
 
@@ -393,6 +399,7 @@ std::tuple<Tensor, Tensor> norm_forward(const Tensor& x, int64_t groups, const T
     s.d.workspace = ptr(ws);
     s.d.workspace_bytes = n;
     check_rc(lib.norm_fwd(&s.d, stream_of(x)), "plc_group_norm_fwd");
+    written(used);
     return {y, stats};
 }
 

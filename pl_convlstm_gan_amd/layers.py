@@ -19,13 +19,14 @@ def gated_linear_scan(x, f, h0=None, lengths=None, coupled=True):
 
     ``h0``: float32 [B, ...], the state in front of the first step (default zeros).  ``lengths``: int32 [B] on x's
     device; behind a sample's length the outputs and gradients are 0, whatever the padding holds, and its state stands
-    still.  Strided x and f are read in place as long as their trailing dimensions are contiguous."""
+    still.  An infinite x makes the states behind it infinite or NaN.  Strided x and f are read in place as long as their trailing dimensions are contiguous."""
     return _lib.binding().scan(x, f, h0, lengths, coupled)
 
 
 def gated_linear_step(x, f, state, coupled=True, inplace=False):
     """One step of gated_linear_scan for serving, without gradients: x, f [B, ...], ``state`` float32 [B, ...];
-    returns (h in x's type, new state).  ``inplace``: the new state overwrites ``state``."""
+    returns (h in x's type, new state).  ``inplace``: the new state overwrites ``state`` (and is an in-place change of it
+    to autograd: a backward pass that needs the old one refuses to run)."""
     return _lib.binding().step(x, f, state, coupled, inplace)
 
 

@@ -242,6 +242,22 @@ def test_scan_pieces_carry_the_state(layers, gpu):
         R.check(q, val[k], err[k], k + " in two pieces")
 
 
+def test_scan_step_in_place_is_seen_by_autograd(layers, gpu):
+    """A state that a backward pass still needs and a step in place overwrites: an error, not a wrong gradient."""
+    x, f = rand((2, 5, 12), 1, torch.float32, gpu).requires_grad_(), rand((2, 5, 12), 2, torch.float32, gpu)
+    h0 = rand((2, 12), 3, torch.float32, gpu)
+    y, _ = layers.gated_linear_scan(x, f, h0)
+    layers.gated_linear_step(f[:, 0], f[:, 1], h0)
+    y.sum().backward(retain_graph=True)
+    layers.gated_linear_step(f[:, 0], f[:, 1], h0, inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    with torch.inference_mode():
+        state = torch.zeros(2, 12, device=gpu)
+        layers.gated_linear_step(f[:, 0], f[:, 1], state, inplace=True)
+        assert torch.equal(state, layers.gated_linear_step(f[:, 0], f[:, 1], torch.zeros(2, 12, device=gpu))[1])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("B,T,D", [(1, 79, 6), (1, 80, 6), (2, 96, 1024), (3, 127, 2048), (3, 250, 2048), (2, 129, 1030), (1, 2100, 40), (1, 9000, 16), (2, 300, 20482)])
 def test_scan_around_the_split(layers, gpu, dtype, B, T, D):
