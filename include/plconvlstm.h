@@ -428,7 +428,8 @@ enum { PLC_F32 = 0, PLC_BF16 = 1, PLC_F16 = 2 };
  * Backward (dh_last, dh0 may be NULL): g_t = dy_t + s_{t+1} g_{t+1}, g behind the last step = dh_last;
  *   coupled: dx_t = (1 - s_t) g_t, df_t = g_t (h_{t-1} - x_t) s_t (1 - s_t);  else dx_t = g_t, df_t = g_t h_{t-1} s_t (1 - s_t);
  *   dh0 = s_0 g_0.  The states are rebuilt in fp32 from x, f and `states`; y is not read.
- * Results do not depend on anything but the inputs and sizes (no atomics).  T = 1 is the single-step form. */
+ * Results depend on the inputs, sizes, strides and alignment alone (no atomics; the latter two choose the width of the
+ * accesses and with it how a long sequence is divided).  T = 1 is the single-step form. */
 typedef struct plc_scan_desc {
     int B, T;
     long long D;

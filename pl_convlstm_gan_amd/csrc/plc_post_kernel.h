@@ -96,8 +96,8 @@ __device__ __forceinline__ void plc_post_pass(const char* lds, int r0, int px, i
 typedef float plc_f32x4_t __attribute__((ext_vector_type(4)));
 
 // Two bf16 products, each rounded to bf16 once: the fp32 product of two bf16 values is exact, so this is what a
-// scalar multiply-and-round of each pair gives.  One packed multiply for the pair (the staging is bound by the
-// number of vector instructions, four cycles each for a 64-lane wave).
+// scalar multiply-and-round of each pair gives.  The rounding of the pair is one instruction (the staging is bound by
+// the number of vector instructions, four cycles each for a 64-lane wave).
 __device__ __forceinline__ unsigned plc_mul_bf2(unsigned x, unsigned y) {
     const plc_f32x2_t xf = {__builtin_bit_cast(float, x << 16), __builtin_bit_cast(float, x & 0xffff0000u)};
     const plc_f32x2_t yf = {__builtin_bit_cast(float, y << 16), __builtin_bit_cast(float, y & 0xffff0000u)};
