@@ -1,9 +1,9 @@
 // Dropout whose mask is computed from a counter instead of being stored: y = keep ? x * scale : 0, plus a residual.
 // The backward pass runs the same kernel on dy.  A dropped element is exactly 0, also where x is not finite.
 // The product and the residual's sum are fp32; y is rounded once.
-// Bound by memory: 84 M bf16 elements 57.7 us (336 MB: 5.8 TB/s); ten rounds of the generator serve eight elements,
+// Bound by memory: 84 M bf16 elements 56.9 us (336 MB: 5.9 TB/s); ten rounds of the generator serve eight elements,
 // so that one lane makes one 16-byte store (8 fp32 elements: two).  Small calls cost their launch: 1 M odd fp16 elements with a
-// residual 2.9 us.
+// residual 3.0 us.
 #pragma once
 #include "plc_layers_common.h"
 
@@ -17,7 +17,7 @@ struct DropoutArgs {
 };
 
 // one lane per call of the generator: eight consecutive elements, moved as vectors of VEC
-template <class T, int VEC>
+template <class T, int VEC, bool STREAM>
 __global__ __launch_bounds__(256) void plc_dropout_kernel(DropoutArgs a) {
     PlcDrop d = a.drop;
     if (a.offset_ptr) d.offset = (uint64_t)*a.offset_ptr;
@@ -28,7 +28,7 @@ __global__ __launch_bounds__(256) void plc_dropout_kernel(DropoutArgs a) {
     T* y = (T*)a.y + e0;
     const uint32_t keep = plc_keep_bits<8>(d, e0);
     if (VEC == 8 && e0 + 8 <= a.n) {
-        const PlcVec<T, 8> v = plc_load<T, 8>(x);
+        const PlcVec<T, 8> v = plc_load<T, 8, STREAM>(x);
         PlcVec<T, 8> w = v;
         if (r) w = plc_load<T, 8>(r);
         float o[8];

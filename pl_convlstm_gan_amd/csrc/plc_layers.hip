@@ -27,6 +27,14 @@ struct VecRule {
         default: CALL(plc_f16); break;      \
     }
 
+// Whether an operator that reads its inputs once reads them past the caches.  It pays for tensors whose inputs and output
+// together do not fit the 256 MB behind the L2s while each alone does: the output stays there, for whoever reads it next.
+// In us, kept against streamed, in brackets with a reader of the output behind it:
+//   scan forward, bf16   84 MB 49.5 (81.8) 53.9 (79.3)   126 MB 83.5 (129) 79.4 (119)   168 MB 110 (167) 97 (150)   335 MB 218 (320) 230 (343)
+//   dropout + residual   84 MB 42.9 (70.8) 44.2 (70.0)   126 MB 69.2 (112) 62.0 (102)   168 MB 91.6 (151) 87.3 (138)   335 MB 177 (286) 168 (291)
+// (Not where a backward pass will read the scan's inputs again: a training pass of 168 MB tensors takes 316 us with it, 309 without.)
+static bool streams(double bytes) { return bytes > 100e6 && bytes < 256e6; }
+
 // ---------------------------------------------------------------------------------------------
 // dropout
 // ---------------------------------------------------------------------------------------------
@@ -60,10 +68,11 @@ extern "C" int plc_dropout(const void* x, const void* residual, void* y, long lo
     a.used_offset = used_offset;
     const long long blocks = (n + 2047) / 2048;
     if (!grid_ok(blocks, 256)) return plc_fail(PLC_EUNSUPPORTED, "dropout: %lld elements are more than one launch covers", n);
-    const bool wide = aligned16(x) && aligned16(y) && aligned16(residual);
+    const bool wide = aligned16(x) && aligned16(y) && aligned16(residual), large = streams((double)n * e);
 #define CALL(T)                                                                                                        \
-    if (wide) hipLaunchKernelGGL((plc_dropout_kernel<T, 8>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a); \
-    else hipLaunchKernelGGL((plc_dropout_kernel<T, 1>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a)
+    if (wide && large) hipLaunchKernelGGL((plc_dropout_kernel<T, 8, sizeof(T) == 2>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a); \
+    else if (wide) hipLaunchKernelGGL((plc_dropout_kernel<T, 8, false>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a); \
+    else hipLaunchKernelGGL((plc_dropout_kernel<T, 1, false>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a)
     PLC_BY_TYPE(dtype, CALL)
 #undef CALL
     PLC_HIP(hipGetLastError());
@@ -174,7 +183,9 @@ static int scan_launch(const ScanArgs& a, hipStream_t st) {
         if (!grid_ok(blocks, 256)) return plc_fail(PLC_EUNSUPPORTED, "gated scan: %lld lanes are more than one launch covers", lanes);
         const dim3 grid((unsigned)blocks), block(256);
         if (BACKWARD) hipLaunchKernelGGL((plc_scan_bwd_kernel<T, V, COUPLED>), grid, block, 0, st, a);
-        else hipLaunchKernelGGL((plc_scan_fwd_kernel<T, V, COUPLED>), grid, block, 0, st, a);
+        else if (V * sizeof(T) == 16 && !a.states && streams((double)a.B * a.T * a.D * sizeof(T)))
+            hipLaunchKernelGGL((plc_scan_fwd_kernel<T, V, COUPLED, V * sizeof(T) == 16>), grid, block, 0, st, a);
+        else hipLaunchKernelGGL((plc_scan_fwd_kernel<T, V, COUPLED, false>), grid, block, 0, st, a);
     }
     PLC_HIP(hipGetLastError());
     return PLC_OK;
@@ -290,7 +301,9 @@ static int norm_plan(const plc_norm_desc* d, bool backward, NormArgs* a, NormPla
     // and rows of less than 64 bytes that are part of longer ones move lines more than once (512 x 30 x 24, fp32, 16-byte rows:
     // 27.9/59.5 against 29.2/46.9).
     const int ku_max = backward ? 8 : 16;
-    const bool large = (double)a->N * (double)a->img * e > 20e6;
+    const double bytes = (double)a->N * (double)a->img * e;
+    const bool large = bytes > 20e6;
+    pl->stream = bytes > 64e6;
     if (a->parts == 1 && m0 <= 64 && d->HW > 0 && (long long)d->HW * m0 <= 512ll * ku_max) {
         int widest = m0;
         if (!a->px_first)

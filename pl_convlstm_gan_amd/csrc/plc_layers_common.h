@@ -35,13 +35,18 @@ struct alignas(V * sizeof(T) > 16 ? 16 : V * sizeof(T)) PlcVec {
     }
 };
 
-template <class T, int V>
+// STREAM: the access does not keep its line in the caches (whole vectors only); for tensors that are too large to be
+// found there again.
+typedef uint32_t plc_u32x4 __attribute__((ext_vector_type(4)));
+template <class T, int V, bool STREAM = false>
 __device__ __forceinline__ PlcVec<T, V> plc_load(const T* p) {
-    return *reinterpret_cast<const PlcVec<T, V>*>(p);
+    if constexpr (STREAM && sizeof(PlcVec<T, V>) == 16) return __builtin_bit_cast(PlcVec<T, V>, __builtin_nontemporal_load(reinterpret_cast<const plc_u32x4*>(p)));
+    else return *reinterpret_cast<const PlcVec<T, V>*>(p);
 }
-template <class T, int V>
+template <class T, int V, bool STREAM = false>
 __device__ __forceinline__ void plc_store(T* p, const PlcVec<T, V>& v) {
-    *reinterpret_cast<PlcVec<T, V>*>(p) = v;
+    if constexpr (STREAM && sizeof(PlcVec<T, V>) == 16) __builtin_nontemporal_store(__builtin_bit_cast(plc_u32x4, v), reinterpret_cast<plc_u32x4*>(p));
+    else *reinterpret_cast<PlcVec<T, V>*>(p) = v;
 }
 template <class T, int V>
 __device__ __forceinline__ void plc_to_float(const PlcVec<T, V>& v, float (&o)[V]) {

@@ -14,11 +14,11 @@
 // the output, one launch.  Split: a first launch writes partial sums over ranges of pixels, the second adds them up
 // (every workgroup for its own groups) and makes the output, reading its inputs a second time.
 //
-// What bounds it: memory.  40 samples of 256 x 256 x 32 bf16, forward: statistics 45.6 us (168 MB: 3.7 TB/s), output 58.2
-// (336 MB: 5.8 TB/s), where one copy of the tensor would take 64; the second reading is the price of a sum over a sample that no
+// What bounds it: memory.  40 samples of 256 x 256 x 32 bf16, forward: statistics 33.9 us (168 MB: 5.0 TB/s), output 51.3
+// (336 MB: 6.5 TB/s), where one copy of the tensor would take 64; the second reading is the price of a sum over a sample that no
 // workgroup holds.  Joining the workgroups of a sample inside one launch (partial sums exchanged through memory) read once and
-// was slower, 157 us against 105, as was going through the tensor in chunks of samples that fit the caches (113 to 182).
-// 80 samples of 128 x 128 x 32 with silu and dropout: 26.6 + 43.4 us forward, 55.6 + 55.4 backward; there the generator (ten
+// was slower, 157 us, as was going through the tensor in chunks of samples that fit the caches (113 to 182).
+// 80 samples of 128 x 128 x 32 with silu and dropout: 20.1 + 43.4 us forward, 56.0 + 54.1 backward; there the generator (ten
 // rounds per eight elements) and the exponential cost as much as the memory.
 // Resident: 5 x 15 x 12 x 32 fp32 3.9 us forward, one launch of 20 workgroups, all latency; 8 x 32 x 32 x 512 fp16 9 us
 // forward (17 MB: 1.9 TB/s) and 15 + 4 backward, the last for dw and db.
@@ -314,7 +314,7 @@ __device__ __forceinline__ void norm_load_stats(const NormArgs& a, const NormBlo
 
 // Calls f(first pixel, number of pixels, loaded units) for rounds of P pixels of a thread; whole rounds carry no conditions,
 // so that all their loads are in flight at once.
-template <class T, int V, int P, int NT, class F>
+template <class T, int V, int P, int NT, bool STREAM, class F>
 __device__ __forceinline__ void norm_rounds(const T* const (&src)[NT], long long ps, int p0, int p1, int rows, F f) {
     PlcVec<T, V> raw[NT][P];
     int p = p0;
@@ -322,7 +322,7 @@ __device__ __forceinline__ void norm_rounds(const T* const (&src)[NT], long long
 #pragma unroll
         for (int j = 0; j < P; ++j)
 #pragma unroll
-            for (int k = 0; k < NT; ++k) raw[k][j] = plc_load<T, V>(src[k] + (long long)(p + j * rows) * ps);
+            for (int k = 0; k < NT; ++k) raw[k][j] = plc_load<T, V, STREAM>(src[k] + (long long)(p + j * rows) * ps);
 #pragma unroll
         for (int j = 0; j < P; ++j) {
             PlcVec<T, V> one[NT];
@@ -338,7 +338,7 @@ __device__ __forceinline__ void norm_rounds(const T* const (&src)[NT], long long
         for (int j = 0; j < P; ++j)
             if (p + j * rows < p1) {
 #pragma unroll
-                for (int k = 0; k < NT; ++k) raw[k][j] = plc_load<T, V>(src[k] + (long long)(p + j * rows) * ps);
+                for (int k = 0; k < NT; ++k) raw[k][j] = plc_load<T, V, STREAM>(src[k] + (long long)(p + j * rows) * ps);
             }
 #pragma unroll
         for (int j = 0; j < P; ++j)
@@ -452,6 +452,9 @@ __device__ __forceinline__ float norm_entry_count(const NormArgs& a, int V, int 
 }
 
 // ---- split form, forward, second pass ---------------------------------------------------------------------------
+// Nothing it touches is needed in the caches afterwards, and what the first pass left of x there is: loads and stores stream.
+// bf16, 32 channels in 8 groups, both passes together: 40 x 256 x 256 86.4 us against 104.4, 20 x 128 x 128 19.5 against 20.6; with
+// an operator that reads y behind them 160 against 172 and 30.5 against 30.9.  (Streaming in the first pass too: 93.8.)
 template <class T, int V, int FORM>
 __global__ __launch_bounds__(256) void plc_norm_fwd_kernel(NormArgs a) {
     extern __shared__ __align__(16) float st[];
@@ -492,8 +495,8 @@ __global__ __launch_bounds__(256) void plc_norm_fwd_kernel(NormArgs a) {
     T* y = (T*)a.y + at;
     const int p0 = blk.range * a.px_split, p1 = min(p0 + a.px_split, a.HW);
     const T* const src[1] = {x};
-    norm_rounds<T, V, NORM_P, 1>(src, a.ps, p0 + t.r, p1, t.rows, [&](int p, const PlcVec<T, V> (&v)[1]) {
-        plc_store<T, V>(y + (long long)p * a.ps, norm_out<T, V, FORM>(a, k, drop, blk.n, p, u, v[0]));
+    norm_rounds<T, V, NORM_P, 1, true>(src, a.ps, p0 + t.r, p1, t.rows, [&](int p, const PlcVec<T, V> (&v)[1]) {
+        plc_store<T, V, true>(y + (long long)p * a.ps, norm_out<T, V, FORM>(a, k, drop, blk.n, p, u, v[0]));
     });
 }
 
@@ -588,7 +591,7 @@ __global__ __launch_bounds__(256) void plc_norm_bwd_sums_kernel(NormArgs a) {
         const long long at = blk.n * a.img + (long long)u * a.us;
         const T *x = (const T*)a.x + at, *dy = (const T*)a.dy + at;
         const T* const src[2] = {x, dy};
-        norm_rounds<T, V, NORM_PB, 2>(src, a.ps, p0 + t.r, p1, t.rows, [&](int p, const PlcVec<T, V> (&q)[2]) {
+        norm_rounds<T, V, NORM_PB, 2, false>(src, a.ps, p0 + t.r, p1, t.rows, [&](int p, const PlcVec<T, V> (&q)[2]) {
             float d[V], dz[V];
             norm_dz<T, V, FORM>(a, k, drop, blk.n, p, u, q[0], q[1], d, dz);
 #pragma unroll
@@ -636,7 +639,9 @@ __global__ __launch_bounds__(256) void plc_norm_params_kernel(NormArgs a) {
 }
 
 // ---- split form, backward, second pass: dx; the leading workgroups sum dw and db -----------------------------------
-template <class T, int V, int FORM>
+// STREAM as in the forward pass, for tensors that the caches do not hold: 40 x 256 x 256 152 us against 174, 80 x 128 x 128 with silu
+// 82 against 88; small ones lose by it (2 x 256 x 256 18.3 against 17.6, with a reader of dx behind it 27.2 against 25.1).
+template <class T, int V, int FORM, bool STREAM>
 __global__ __launch_bounds__(256) void plc_norm_bwd_kernel(NormArgs a) {
     extern __shared__ __align__(16) float lds[];
     if ((int)blockIdx.x < a.param_blocks) {
@@ -678,10 +683,10 @@ __global__ __launch_bounds__(256) void plc_norm_bwd_kernel(NormArgs a) {
     T* dx = (T*)a.dx + at;
     const int p0 = blk.range * a.px_split, p1 = min(p0 + a.px_split, a.HW);
     const T* const src[2] = {x, dy};
-    norm_rounds<T, V, NORM_PB, 2>(src, a.ps, p0 + t.r, p1, t.rows, [&](int p, const PlcVec<T, V> (&v)[2]) {
+    norm_rounds<T, V, NORM_PB, 2, STREAM>(src, a.ps, p0 + t.r, p1, t.rows, [&](int p, const PlcVec<T, V> (&v)[2]) {
         float d[V], dz[V];
         norm_dz<T, V, FORM>(a, k, drop, blk.n, p, u, v[0], v[1], d, dz);
-        plc_store<T, V>(dx + (long long)p * a.ps, norm_dx<T, V>(k, q, d, dz));
+        plc_store<T, V, STREAM>(dx + (long long)p * a.ps, norm_dx<T, V>(k, q, d, dz));
     });
 }
 

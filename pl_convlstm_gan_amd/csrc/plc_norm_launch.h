@@ -7,6 +7,7 @@
 struct NormPlan {
     int v;               // channels of a unit
     int ku, threads;     // resident form: units of a thread (0: split form), threads of a workgroup
+    bool stream;         // split form: the tensors are larger than what the caches keep between two passes
     size_t part_g, part_c, total;     // workspace
 };
 
@@ -39,7 +40,9 @@ int norm_launch(NormArgs a, const NormPlan& pl, bool backward, hipStream_t st) {
         hipLaunchKernelGGL((plc_norm_bwd_sums_kernel<T, V, FORM>), dim3(blocks), dim3(256), (3 * nch + norm_lds_floats(256, a.ut, V, 1)) * f, st, a);
         a.param_blocks = params;
         const int lds = 4 * nch * f, need = 512 * (int)sizeof(double);
-        hipLaunchKernelGGL((plc_norm_bwd_kernel<T, V, FORM>), dim3(blocks + params), dim3(256), lds < need ? need : lds, st, a);
+        const dim3 grid(blocks + params);
+        if (V * sizeof(T) == 16 && pl.stream) hipLaunchKernelGGL((plc_norm_bwd_kernel<T, V, FORM, V * sizeof(T) == 16>), grid, dim3(256), lds < need ? need : lds, st, a);
+        else hipLaunchKernelGGL((plc_norm_bwd_kernel<T, V, FORM, false>), grid, dim3(256), lds < need ? need : lds, st, a);
     }
     PLC_HIP(hipGetLastError());
     return PLC_OK;

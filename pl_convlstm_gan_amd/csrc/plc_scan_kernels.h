@@ -6,7 +6,7 @@
 //
 // What bounds it: memory, once there are rows enough.  Forward 3 tensors of B T D elements plus a state every SCAN_K steps,
 // backward 5.  8 x 10 x 128 x 128 x 32 bf16 forward without states 47 us, 285 MB: 6.1 TB/s (a large copy runs at 5.2, reading
-// alone at 6 to 7).  4 x 10 x 256 x 256 x 32 bf16 forward with states 120 us (600 MB), backward 195 us (873 MB): 5.0 and 4.5 TB/s.
+// alone at 6 to 7).  4 x 10 x 256 x 256 x 32 bf16 forward with states 122 us (604 MB), backward 196 us (973 MB): 5.0 TB/s both.
 #pragma once
 #include "plc_layers_common.h"
 
@@ -83,21 +83,21 @@ __device__ __forceinline__ void scan_load_state(const float* p, long long at, fl
 // Rows t0 .. t0 + SCAN_K - 1 of one tensor.  Not FULL: the block reaches behind some lane's sample.  Its loads are not
 // conditional all the same (they would wait for one another); a row behind the sequence becomes its last one, which is
 // memory of the tensor, and what is loaded there is not used.
-template <class T, int V, bool FULL>
+template <class T, int V, bool FULL, bool STREAM = false>
 __device__ __forceinline__ void scan_rows(const ScanArgs& a, const void* base, long long sb, long long st, const ScanLane& l, int t0, PlcVec<T, V> (&r)[SCAN_K]) {
     const T* p = (const T*)base + l.b * sb + l.d + t0 * st;
     const int most = a.T - 1 - t0;
 #pragma unroll
-    for (int j = 0; j < SCAN_K; ++j) r[j] = plc_load<T, V>(p + (FULL ? j : min(j, most)) * st);
+    for (int j = 0; j < SCAN_K; ++j) r[j] = plc_load<T, V, STREAM>(p + (FULL ? j : min(j, most)) * st);
 }
 
 // ---- forward ----------------------------------------------------------------------------------------------------
 // one block of steps from state h; rows between the sample's length and T get 0
-template <class T, int V, bool COUPLED, bool FULL>
+template <class T, int V, bool COUPLED, bool FULL, bool STREAM>
 __device__ __forceinline__ void scan_fwd_block(const ScanArgs& a, const ScanLane& l, int t0, float (&h)[V]) {
     PlcVec<T, V> xr[SCAN_K], fr[SCAN_K];
-    scan_rows<T, V, FULL>(a, a.f, a.f_sb, a.f_st, l, t0, fr);
-    scan_rows<T, V, FULL>(a, a.x, a.x_sb, a.x_st, l, t0, xr);
+    scan_rows<T, V, FULL, STREAM>(a, a.f, a.f_sb, a.f_st, l, t0, fr);
+    scan_rows<T, V, FULL, STREAM>(a, a.x, a.x_sb, a.x_st, l, t0, xr);
     T* y = (T*)a.y + (l.b * a.T + t0) * a.D + l.d;
 #pragma unroll
     for (int j = 0; j < SCAN_K; ++j) {
@@ -124,26 +124,26 @@ __device__ __forceinline__ void scan_zero_block(const ScanArgs& a, T* y, const S
     for (int j = 0; j < SCAN_K; ++j)
         if (t0 + j < a.T) plc_store<T, V>(y + j * a.D, plc_from_float<T, V>(o));
 }
-template <class T, int V, bool COUPLED>
+template <class T, int V, bool COUPLED, bool STREAM>
 __device__ __forceinline__ void scan_fwd_range(const ScanArgs& a, const ScanLane& l, int t0, int t1, float (&h)[V]) {
     const int blocks = (a.T + SCAN_K - 1) / SCAN_K;
     for (int t = t0; t < t1; t += SCAN_K) {
         const int k = t / SCAN_K;
         if (k > 0 && a.states) plc_store<float, V>(a.states + (l.b * (blocks - 1) + k - 1) * a.D + l.d, plc_from_float<float, V>(h));
-        if (__all(t + SCAN_K <= l.n)) scan_fwd_block<T, V, COUPLED, true>(a, l, t, h);
-        else if (__any(t < l.n)) scan_fwd_block<T, V, COUPLED, false>(a, l, t, h);
+        if (__all(t + SCAN_K <= l.n)) scan_fwd_block<T, V, COUPLED, true, STREAM>(a, l, t, h);
+        else if (__any(t < l.n)) scan_fwd_block<T, V, COUPLED, false, STREAM>(a, l, t, h);
         else scan_zero_block<T, V>(a, (T*)a.y, l, t);
     }
 }
 
-// one lane from the first step to the last
-template <class T, int V, bool COUPLED>
+// one lane from the first step to the last; STREAM: x and f do not stay in the caches
+template <class T, int V, bool COUPLED, bool STREAM>
 __global__ __launch_bounds__(256) void plc_scan_fwd_kernel(ScanArgs a) {
     ScanLane l;
     if (!scan_lane<V>(a, (long long)blockIdx.x * blockDim.x + threadIdx.x, l)) return;
     float h[V];
     scan_load_state<V>(a.h0, l.b * a.D + l.d, h);
-    scan_fwd_range<T, V, COUPLED>(a, l, 0, a.T, h);
+    scan_fwd_range<T, V, COUPLED, STREAM>(a, l, 0, a.T, h);
     if (a.h_last) plc_store<float, V>(a.h_last + l.b * a.D + l.d, plc_from_float<float, V>(h));
 }
 
@@ -341,7 +341,7 @@ __global__ __launch_bounds__(256) void plc_scan_split_kernel(ScanArgs a) {
         scan_bwd_range<T, V, COUPLED>(a, l, t0, t1, h);
         if (k == 0 && a.dh0) plc_store<float, V>(a.dh0 + l.b * a.D + l.d, plc_from_float<float, V>(h));
     } else {
-        scan_fwd_range<T, V, COUPLED>(a, l, t0, t1, h);
+        scan_fwd_range<T, V, COUPLED, false>(a, l, t0, t1, h);
         if (k == a.nseg - 1 && a.h_last) plc_store<float, V>(a.h_last + l.b * a.D + l.d, plc_from_float<float, V>(h));
     }
 }
