@@ -6,6 +6,7 @@
 // Python autograd functions and ctypes, of which the kernels were 10 to 30 us.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
@@ -251,11 +252,32 @@ struct ScanFn : public torch::autograd::Function<ScanFn> {
     }
 };
 
+// A leaf's accumulation node lives as long as any autograd graph that uses the leaf, and belongs to the stream that graph was
+// made on.  A backward pass that is being captured and reaches such a node pulls that stream into the capture, which ends
+// the process when the capture ends: refused here, while it can be.
+void check_captured(const Tensor& t) {
+    if (!t.is_leaf() || !t.is_cuda()) return;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (!node) return;
+    // (by id: autograd's streams and these name the device's type differently)
+    const auto here = c10::hip::getCurrentHIPStream(t.device().index()).id();
+    const auto made = node->stream();
+    TORCH_CHECK(!made.has_value() || made->id() == here, "a graph is being captured while outputs of an earlier pass over the same leaf tensor are alive: "
+                "its gradient would be accumulated on that pass's stream.  Detach or delete those outputs first.");
+}
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
     if (!at::GradMode::is_enabled()) return false;
+    const Tensor* any = nullptr;
     for (const Tensor* t : ts)
-        if (t->defined() && t->requires_grad()) return true;
-    return false;
+        if (t->defined() && t->requires_grad()) any = t;
+    if (!any) return false;
+    if (any->is_cuda()) {
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing(c10::hip::getCurrentHIPStream(any->device().index()).stream(), &status) == hipSuccess && status != hipStreamCaptureStatusNone)
+            for (const Tensor* t : ts)
+                if (t->defined() && t->requires_grad()) check_captured(*t);
+    }
+    return true;
 }
 
 std::tuple<Tensor, Tensor> scan(const Tensor& x, const Tensor& f, const OptTensor& h0, const OptTensor& lengths, bool coupled) {

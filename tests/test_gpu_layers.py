@@ -378,7 +378,7 @@ def test_norm_shapes(layers, gpu, shape, groups, dtype):
 
 
 @pytest.mark.parametrize("shape,groups,dtype", [((256, 32, 30, 24), 8, torch.float32), ((256, 32, 41, 40), 1, torch.bfloat16), ((640, 32, 23, 23), 8, torch.float16),
-                                                ((530, 24, 30, 31), 3, torch.bfloat16), ((40, 512, 23, 24), 32, torch.float16)])
+                                                ((530, 24, 30, 31), 3, torch.bfloat16), ((40, 512, 23, 24), 32, torch.float16), ((16, 32, 256, 257), 8, torch.bfloat16)])
 def test_norm_beyond_the_caches(layers, gpu, shape, groups, dtype):
     """More than 20 MB in many small samples, where the choice between the forms is another one."""
     norm_case(layers, gpu, shape, groups, dtype, "silu")
@@ -522,6 +522,36 @@ def test_block_captured_and_replayed(layers, gpu):
         torch.randn(1000, device=gpu).sum().item()
 
 
+def test_capture_beside_a_live_eager_graph_is_refused(layers, gpu):
+    """Outputs of an eager pass over the same leaves are alive when a training pass is captured: an error at the first
+    operator; once they are dropped the capture works."""
+    def calls(m):
+        x = rand((2, 16, 8, 8), 1, torch.float32, gpu).contiguous(memory_format=torch.channels_last)
+        return {"norm": lambda: layers.group_norm_act(x, 4, m["w"], m["b"]),
+                "scan": lambda: layers.gated_linear_scan(m["s"], m["s"])[0],
+                "dropout": lambda: layers.counter_dropout(m["s"], 0.5, 1)}
+    leaves = {"w": torch.ones(16, device=gpu, requires_grad=True), "b": torch.zeros(16, device=gpu, requires_grad=True),
+              "s": rand((2, 20, 12), 3, torch.float32, gpu).requires_grad_()}
+    for name, call in calls(leaves).items():
+        call()                                            # (its graph is dropped with it)
+        want = torch.autograd.grad(call().sum(), [t for t in leaves.values()], allow_unused=True)
+        alive = call()
+        with pytest.raises(RuntimeError, match="earlier pass over the same leaf"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+        with torch.no_grad(), torch.cuda.graph(torch.cuda.CUDAGraph()):
+            call()                                        # (no gradients, no difficulty)
+        del alive
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = torch.autograd.grad(call().sum(), [t for t in leaves.values()], allow_unused=True)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            for p, q in zip(got, want):
+                assert (p is None and q is None) or torch.equal(p, q), name
+
+
 def test_modules(layers, gpu):
     m = layers.GroupNormAct(4, 16, act="relu", p=0.3, seed=9).to(gpu)
     x = rand((2, 16, 8, 8), 1, torch.float32, gpu).contiguous(memory_format=torch.channels_last)
@@ -624,3 +654,17 @@ def test_offsets_beyond_32_bits(layers, gpu):
     z = layers.group_norm_act(x, 4, act="relu", p=0.5, seed=1)[2].permute(1, 2, 0).reshape(-1)
     keep = layers.counter_dropout(torch.ones(3 * 4700 * 4800 * 32, dtype=torch.bfloat16, device=gpu), 0.5, 1)[-z.numel():] != 0
     assert float(z[~keep].abs().max()) == 0 and torch.equal(z[keep], (y[2].permute(1, 2, 0).reshape(-1)[keep].float() * 2).to(torch.bfloat16))
+
+
+def test_large_tensors_streamed_past_the_caches(layers, gpu):
+    """Sizes at which inputs are read past the caches: the bits of the calls that keep them there."""
+    x, f = rand((1, 10, 6000008), 1, torch.bfloat16, gpu), rand((1, 10, 6000008), 2, torch.bfloat16, gpu)
+    y, h = layers.gated_linear_scan(x, f)
+    g = x.detach().requires_grad_()                       # (a training pass does not stream)
+    y2, h2 = layers.gated_linear_scan(g, f)
+    assert torch.equal(y, y2) and torch.equal(h, h2)
+    # dropout: fp32 tensors are never streamed; same mask, the same product, rounded once
+    out = layers.counter_dropout(x, 0.3, 5, 6, residual=f)
+    assert torch.equal(out, layers.counter_dropout(x.float(), 0.3, 5, 6, residual=f.float()).bfloat16())
+    out = layers.counter_dropout(x, 0.3, 5, 6)
+    assert torch.equal(out, layers.counter_dropout(x.float(), 0.3, 5, 6).bfloat16())
