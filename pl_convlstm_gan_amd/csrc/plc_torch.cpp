@@ -7,6 +7,7 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
@@ -265,7 +266,15 @@ void check_captured(const Tensor& t) {
     TORCH_CHECK(!made.has_value() || made->id() == here, "a graph is being captured while outputs of an earlier pass over the same leaf tensor are alive: "
                 "its gradient would be accumulated on that pass's stream.  Detach or delete those outputs first.");
 }
+// There are no forward-mode derivatives: a tensor that carries a tangent is refused, since the result would carry none.
+void check_no_tangent(std::initializer_list<const Tensor*> ts) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor* t : ts)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(),
+                                    "forward-mode derivatives of the layer operators are not available");
+}
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
+    check_no_tangent(ts);
     if (!at::GradMode::is_enabled()) return false;
     const Tensor* any = nullptr;
     for (const Tensor* t : ts)
@@ -291,6 +300,7 @@ std::tuple<Tensor, Tensor> scan(const Tensor& x, const Tensor& f, const OptTenso
 }
 
 std::tuple<Tensor, Tensor> scan_one_step(const Tensor& x_, const Tensor& f_, const Tensor& state_, bool coupled, bool inplace) {
+    check_no_tangent({&x_, &f_, &state_});
     const at::AutoGradMode off(false);
     const Tensor x = x_.detach(), f = f_.detach(), state = state_.detach();
     dtype_of(x, "x");

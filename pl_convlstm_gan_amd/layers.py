@@ -3,8 +3,9 @@ activation on channels-last tensors, and dropout whose mask is computed from a c
 
 None has a counterpart in the reference.  All are HIP kernels of libplconvlstm (include/plconvlstm.h, "Layer
 operators"); float32, bfloat16 and float16 tensors, states, statistics and sums in float32.  They are differentiable
-once, run on the current stream of their tensors' device, and can be captured into a HIP graph (a training pass only
-while no output of an earlier pass over the same leaf tensors is alive: that raises).
+once, in reverse mode (a tensor with a forward-mode tangent raises), run on the current stream of their tensors' device,
+and can be captured into a HIP graph (a training pass only while no output of an earlier pass over the same leaf tensors
+is alive: that raises).
 """
 from __future__ import annotations
 
