@@ -7,8 +7,10 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
 #include "../../include/plconvlstm.h"
@@ -53,6 +55,13 @@ void check_rc(int rc, const char* what) {
     TORCH_CHECK_NOT_IMPLEMENTED(rc != PLC_EUNSUPPORTED, what, ": ", msg);
     TORCH_CHECK_VALUE(rc != PLC_EINVAL, what, ": ", msg);
     TORCH_CHECK(false, what, " failed (code ", rc, "): ", msg);
+}
+
+// A recorder of PyTorch's own operations sees the allocation of a result and not the kernel that fills it: what it made of
+// such a call would return memory that nothing has written.
+void check_not_recorded() {
+    TORCH_CHECK(!torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+                "the layer operators cannot be recorded by torch.jit.trace or torch.fx: their kernels are not PyTorch operations (a HIP graph captures them)");
 }
 
 void on_gpu(const Tensor& t, const char* name) {
@@ -168,6 +177,7 @@ struct Scan {
 
 std::tuple<Tensor, Tensor, Tensor> scan_forward(const Tensor& x, const Tensor& f, const Tensor& h0, const Tensor& lengths, bool coupled,
                                                 bool save_states, const Tensor& into) {
+    check_not_recorded();
     Scan s(x, f, h0, lengths, coupled);
     const c10::OptionalDeviceGuard guard(x.device());
     const auto f32 = x.options().dtype(at::kFloat);
@@ -194,6 +204,7 @@ std::tuple<Tensor, Tensor, Tensor> scan_forward(const Tensor& x, const Tensor& f
 
 std::tuple<Tensor, Tensor, Tensor> scan_backward(const Tensor& x, const Tensor& f, const Tensor& h0, const Tensor& lengths, bool coupled,
                                                  const Tensor& states, const Tensor& dy_, const Tensor& dh_, bool need_dh0) {
+    check_not_recorded();
     Scan s(x, f, h0, lengths, coupled);
     const c10::OptionalDeviceGuard guard(x.device());
     const auto f32 = x.options().dtype(at::kFloat);
@@ -327,6 +338,7 @@ struct Draw {          // what a mask is made of; offset_t: an int64 on the devi
 };
 
 Tensor dropout_forward(const Tensor& x_, double p, uint64_t seed, uint64_t offset, const Tensor& offset_t, const Tensor& residual, const Tensor& used) {
+    check_not_recorded();
     const int dtype = dtype_of(x_, "x");
     const Draw w(p, seed, offset, offset_t, x_);
     const c10::OptionalDeviceGuard guard(x_.device());
@@ -417,6 +429,7 @@ Tensor channels_last_like(const Tensor& x) { return at::empty(x.sizes(), x.optio
 
 std::tuple<Tensor, Tensor> norm_forward(const Tensor& x, int64_t groups, const Tensor& w, const Tensor& b, double eps, int64_t act, double p,
                                         uint64_t seed, uint64_t offset, const Tensor& offset_t, const Tensor& used) {
+    check_not_recorded();
     dtype_of(x, "x");
     const Draw draw(p, seed, offset, offset_t, x);
     const c10::OptionalDeviceGuard guard(x.device());
@@ -437,6 +450,7 @@ std::tuple<Tensor, Tensor> norm_forward(const Tensor& x, int64_t groups, const T
 
 std::tuple<Tensor, Tensor, Tensor> norm_backward(const Tensor& x, int64_t groups, const Tensor& w, const Tensor& b, double eps, int64_t act, double p,
                                                  uint64_t seed, uint64_t offset, const Tensor& offset_t, const Tensor& stats, const Tensor& dy_) {
+    check_not_recorded();
     dtype_of(x, "x");
     const Draw draw(p, seed, offset, offset_t, x);
     const c10::OptionalDeviceGuard guard(x.device());

@@ -31,3 +31,25 @@ def test_forward_mode_derivatives_are_refused(mode):
         for call in calls(x, image).values():
             with pytest.raises(RuntimeError, match="no CPU fallback"):
                 call()
+
+
+@pytest.mark.filterwarnings("ignore")
+def test_recorders_that_cannot_see_a_kernel_are_refused():
+    """torch.jit.trace and make_fx record PyTorch's own operations: of a call of these operators they would keep the
+    allocation of the result and nothing that fills it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from pl_convlstm_gan_amd import ops
+    x, image = torch.randn(2, 3, 4), torch.randn(2, 4, 3, 3)
+    one = lambda k: lambda x, image: calls(x, image)[k]()  # noqa: E731
+    for grad in (False, True):
+        for call in {**{k: one(k) for k in calls(x, image)},
+                           "scan pass": lambda x, image: ops.gated_scan_forward(x, x),
+                           "scan backward pass": lambda x, image: ops.gated_scan_backward(x, x, None, None, True, None, x, None),
+                           "dropout pass": lambda x, image: ops.dropout_forward(x, 0.5, 1),
+                           "norm pass": lambda x, image: ops.group_norm_forward(image, 2),
+                           "norm backward pass": lambda x, image: ops.group_norm_backward(image, 2, None, None, 1e-5, "none", 0.0, 0, 0, x, image)}.values():
+            a, b = x.clone().requires_grad_(grad), image.clone().requires_grad_(grad)
+            with pytest.raises(RuntimeError, match="record"):
+                torch.jit.trace(call, (a, b), check_trace=False)
+            with pytest.raises(RuntimeError, match="record"):
+                make_fx(call)(a, b)
