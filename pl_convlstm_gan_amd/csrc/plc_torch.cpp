@@ -312,6 +312,7 @@ std::tuple<Tensor, Tensor> scan(const Tensor& x, const Tensor& f, const OptTenso
 
 std::tuple<Tensor, Tensor> scan_one_step(const Tensor& x_, const Tensor& f_, const Tensor& state_, bool coupled, bool inplace) {
     check_no_tangent({&x_, &f_, &state_});
+    check_not_recorded();
     const at::AutoGradMode off(false);
     const Tensor x = x_.detach(), f = f_.detach(), state = state_.detach();
     dtype_of(x, "x");
