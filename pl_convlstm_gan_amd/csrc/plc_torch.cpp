@@ -265,17 +265,18 @@ struct ScanFn : public torch::autograd::Function<ScanFn> {
 };
 
 // A leaf's accumulation node lives as long as any autograd graph that uses the leaf, and belongs to the stream that graph was
-// made on.  A backward pass that is being captured and reaches such a node pulls that stream into the capture, which ends
-// the process when the capture ends: refused here, while it can be.
+// made on.  Where that is the default stream, which cannot be captured, a backward pass that is being captured and reaches
+// the node ends the process when the capture ends: refused here, while it can be.  (Another stream joins the capture and is
+// joined again: that works, and is what a warm-up on a side stream leaves behind.)
 void check_captured(const Tensor& t) {
     if (!t.is_leaf() || !t.is_cuda()) return;
     const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
     if (!node) return;
     // (by id: autograd's streams and these name the device's type differently)
-    const auto here = c10::hip::getCurrentHIPStream(t.device().index()).id();
     const auto made = node->stream();
-    TORCH_CHECK(!made.has_value() || made->id() == here, "a graph is being captured while outputs of an earlier pass over the same leaf tensor are alive: "
-                "its gradient would be accumulated on that pass's stream.  Detach or delete those outputs first.");
+    TORCH_CHECK(!made.has_value() || made->id() != c10::hip::getDefaultHIPStream(t.device().index()).id(),
+                "a graph is being captured while outputs of an earlier pass over the same leaf tensor, on the default stream, are alive: "
+                "its gradient would be accumulated there.  Detach or delete those outputs first.");
 }
 // There are no forward-mode derivatives: a tensor that carries a tangent is refused, since the result would carry none.
 void check_no_tangent(std::initializer_list<const Tensor*> ts) {
