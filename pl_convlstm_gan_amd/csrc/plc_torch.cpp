@@ -13,6 +13,8 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
+#include <unordered_set>
+
 #include "../../include/plconvlstm.h"
 
 namespace {
@@ -109,6 +111,42 @@ torch::autograd::variable_list once(torch::autograd::variable_list grads, const 
     for (Tensor& g : grads) in.push_back(g.defined() ? g.detach().requires_grad_() : g);
     torch::autograd::DelayedError err(std::string("second derivatives of ") + what + " are not available", (int64_t)in.size());
     return err.apply(std::move(in));
+}
+
+// A leaf's accumulation node lives as long as any autograd graph that uses the leaf, and belongs to the stream that graph was
+// made on.  Where that is the default stream, which cannot be captured, a backward pass that is being captured and reaches
+// the node ends the process when the capture ends: refused here, while it can be.  (Another stream joins the capture and is
+// joined again: that works, and is what a warm-up on a side stream leaves behind.)
+//
+// The forward call looks through what was computed during the capture (and leads, if anything does, into the captured
+// backward pass) down to the leaves.  A graph made on the default stream before the capture may stay outside that pass, so it is
+// looked at when a backward pass of these operators is about to lead there.
+bool capturing(const c10::hip::HIPStream& stream) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    return hipStreamIsCapturing(stream.stream(), &status) == hipSuccess && status != hipStreamCaptureStatusNone;
+}
+void check_captured(std::vector<torch::autograd::Node*> nodes, int device, bool in_backward) {
+    const auto fixed = c10::hip::getDefaultHIPStream(device).id();       // (by id: autograd's streams name the device's type differently)
+    std::unordered_set<torch::autograd::Node*> seen;
+    while (!nodes.empty()) {
+        torch::autograd::Node* n = nodes.back();
+        nodes.pop_back();
+        if (!seen.insert(n).second) continue;
+        const auto made = n->stream();
+        if (made.has_value() && made->device_index() == device && made->id() == fixed) {
+            TORCH_CHECK(n->num_outputs() > 0 && !in_backward,
+                        "a graph is being captured while outputs of an earlier pass over the same leaf tensor, on the default stream, are alive: "
+                        "its gradient would be accumulated there.  Detach or delete those outputs first.");
+            continue;
+        }
+        for (uint32_t i = 0; i < n->num_outputs(); ++i)
+            if (n->next_edge(i).is_valid() && (!in_backward || n->task_should_compute_output(i))) nodes.push_back(n->next_edge(i).function.get());
+    }
+}
+// called by the backward pass of an operator on a tensor of that device, before it launches anything
+void check_captured_backward(const Tensor& g) {
+    if (!g.is_cuda() || !capturing(c10::hip::getCurrentHIPStream(g.device().index()))) return;
+    if (const auto node = torch::autograd::get_current_node()) check_captured({node.get()}, g.device().index(), true);
 }
 
 // ---------------------------------------------------------------------------------------------- gated recurrence
@@ -252,6 +290,7 @@ struct ScanFn : public torch::autograd::Function<ScanFn> {
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
         if (!g[0].defined() && !g[1].defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+        check_captured_backward(g[0].defined() ? g[0] : g[1]);
         const auto s = ctx->get_saved_variables();
         torch::autograd::variable_list out;
         {
@@ -264,20 +303,6 @@ struct ScanFn : public torch::autograd::Function<ScanFn> {
     }
 };
 
-// A leaf's accumulation node lives as long as any autograd graph that uses the leaf, and belongs to the stream that graph was
-// made on.  Where that is the default stream, which cannot be captured, a backward pass that is being captured and reaches
-// the node ends the process when the capture ends: refused here, while it can be.  (Another stream joins the capture and is
-// joined again: that works, and is what a warm-up on a side stream leaves behind.)
-void check_captured(const Tensor& t) {
-    if (!t.is_leaf() || !t.is_cuda()) return;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
-    if (!node) return;
-    // (by id: autograd's streams and these name the device's type differently)
-    const auto made = node->stream();
-    TORCH_CHECK(!made.has_value() || made->id() != c10::hip::getDefaultHIPStream(t.device().index()).id(),
-                "a graph is being captured while outputs of an earlier pass over the same leaf tensor, on the default stream, are alive: "
-                "its gradient would be accumulated there.  Detach or delete those outputs first.");
-}
 // There are no forward-mode derivatives: a tensor that carries a tangent is refused, since the result would carry none.
 void check_no_tangent(std::initializer_list<const Tensor*> ts) {
     if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
@@ -292,11 +317,16 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
     for (const Tensor* t : ts)
         if (t->defined() && t->requires_grad()) any = t;
     if (!any) return false;
-    if (any->is_cuda()) {
-        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-        if (hipStreamIsCapturing(c10::hip::getCurrentHIPStream(any->device().index()).stream(), &status) == hipSuccess && status != hipStreamCaptureStatusNone)
-            for (const Tensor* t : ts)
-                if (t->defined() && t->requires_grad()) check_captured(*t);
+    if (any->is_cuda() && capturing(c10::hip::getCurrentHIPStream(any->device().index()))) {
+        std::vector<torch::autograd::Node*> nodes;
+        std::vector<std::shared_ptr<torch::autograd::Node>> kept;
+        for (const Tensor* t : ts)
+            if (t->defined() && t->requires_grad())
+                if (auto node = t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn()) {
+                    nodes.push_back(node.get());
+                    kept.push_back(std::move(node));
+                }
+        check_captured(std::move(nodes), any->device().index(), false);
     }
     return true;
 }
@@ -374,6 +404,7 @@ struct DropoutFn : public torch::autograd::Function<DropoutFn> {
         return y;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+        check_captured_backward(g[0]);
         Tensor dx;
         if (ctx->saved_data["dx"].toBool()) {
             const at::AutoGradMode off(false);
@@ -494,6 +525,7 @@ struct NormFn : public torch::autograd::Function<NormFn> {
         return y;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+        check_captured_backward(g[0]);
         const auto s = ctx->get_saved_variables();
         auto& d = ctx->saved_data;
         torch::autograd::variable_list out(10);

@@ -5,7 +5,7 @@ None has a counterpart in the reference.  All are HIP kernels of libplconvlstm (
 operators"); float32, bfloat16 and float16 tensors, states, statistics and sums in float32.  They are differentiable
 once, in reverse mode (a tensor with a forward-mode tangent raises), run on the current stream of their tensors' device,
 and can be captured into a HIP graph (a training pass only while no output of an earlier pass over the same leaf tensors
-on the default stream is alive: that raises).  torch.jit.trace and torch.fx cannot record them: that raises too.
+on the default stream is alive, wherever between the leaves and the loss the operators are: that raises).  torch.jit.trace and torch.fx cannot record them: that raises too.
 """
 from __future__ import annotations
 

@@ -47,3 +47,41 @@ def test_warm_up_on_a_side_stream_may_stay_alive(layers, gpu):
     with torch.cuda.graph(graph):
         _, got = step()
     replays(graph, got, [g.detach() for g in step()[1]])
+
+
+def test_leaves_behind_other_operations(layers, gpu):
+    """The leaf that an earlier pass on the default stream still holds reaches the operator through a cast, a view or another
+    operation: refused like a leaf that is its argument.  Without that pass the capture works."""
+    image = rand((2, 16, 8, 8), 1, torch.float32, gpu).contiguous(memory_format=torch.channels_last)
+    w, s = torch.ones(16, device=gpu, dtype=torch.bfloat16, requires_grad=True), rand((2, 20, 12), 3, torch.float32, gpu).requires_grad_()
+    for name, leaf, call in (("cast weight", w, lambda: layers.group_norm_act(image, 4, w.float())), ("scaled input", s, lambda: layers.gated_linear_scan(s * 2, s.detach())[0]),
+                             ("view", s, lambda: layers.counter_dropout(s[:, 3:], 0.5, 1)), ("gate of a gate", s, lambda: layers.gated_linear_scan(s.detach(), layers.counter_dropout(s, 0.5, 2))[0])):
+        call()
+        (want,) = torch.autograd.grad(call().sum(), leaf)
+        alive = call()
+        with pytest.raises(RuntimeError, match="earlier pass over the same leaf"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+        del alive
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            (got,) = torch.autograd.grad(call().sum(), leaf)
+        replays(graph, [got], [want], name)
+
+
+def test_inputs_computed_before_the_capture(layers, gpu):
+    """An input with a graph of its own, made on the default stream before the capture: gradients that do not lead there are
+    captured, one that does is refused in the backward pass."""
+    base = rand((2, 16, 8, 8), 1, torch.float32, gpu).contiguous(memory_format=torch.channels_last).requires_grad_()
+    w, dy = torch.ones(16, device=gpu, requires_grad=True), rand((2, 16, 8, 8), 2, torch.float32, gpu)
+    x = base * 2
+    want = torch.autograd.grad(layers.group_norm_act(x, 4, w), w, dy)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(layers.group_norm_act(x, 4, w), w, dy)
+    replays(graph, got, want)
+    for into in (base, x):
+        with pytest.raises(RuntimeError, match="earlier pass over the same leaf"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                torch.autograd.grad(layers.group_norm_act(x, 4, w), into, dy)
+    replays(graph, got, want)
