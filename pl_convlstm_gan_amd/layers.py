@@ -39,7 +39,7 @@ def counter_dropout(x, p, seed, offset=0, residual=None):
 
     Calls that must not share a mask take different offsets.  ``offset`` is an integer or an int64 tensor of one element on
     x's device that the kernel reads when it runs: a captured graph that advances it draws a new mask on every replay
-    (the backward pass keeps the value its forward pass used)."""
+    (the backward pass keeps the value its forward pass used; a pass that is recomputed reads it again)."""
     seed, offset, offset_t = ops._draw(seed, offset)
     return _lib.binding().dropout(x, p, seed, offset, offset_t, residual)
 
@@ -53,9 +53,24 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
     return _lib.binding().norm(x, num_groups, weight, bias, eps, ops._act(act), p, seed, offset, offset_t)
 
 
+def _next_offset(module, offset):
+    """The offset of a module's pass: the caller's, or the module's own, of which a pass that runs a second time inside the
+    backward pass would read another value than the first time."""
+    if offset is not None:
+        return offset
+    if ops._inside_backward():
+        raise RuntimeError(f"{type(module).__name__} with dropout runs inside a backward pass (activation recomputation?), where its own "
+                           "offset has moved on and the mask would be another one: give forward() the offset of the pass")
+    return module.offset
+
+
 class GroupNormAct(nn.Module):
     """group_norm_act with its parameters; ``p``: dropout of the training mode.  The dropout's offset is a buffer that
-    every training pass advances by one on the device, so passes draw different masks, replays of a captured pass too."""
+    every training pass advances by one on the device, so passes draw different masks, replays of a captured pass too.
+
+    Where a pass is recomputed (torch.utils.checkpoint), give ``forward`` the ``offset`` of the pass, an integer or an int64 tensor
+    that nothing changes before the backward pass is done; the buffer is then neither read nor advanced.  Without it a
+    recomputation raises: the buffer has moved on by then."""
 
     def __init__(self, num_groups, num_channels, act="none", p=0.0, eps=1e-5, affine=True, seed=0):
         super().__init__()
@@ -64,11 +79,12 @@ class GroupNormAct(nn.Module):
         self.bias = nn.Parameter(torch.zeros(num_channels)) if affine else None
         self.register_buffer("offset", torch.zeros(1, dtype=torch.int64))
 
-    def forward(self, x):
+    def forward(self, x, offset=None):
         p = self.p if self.training else 0.0
-        y = group_norm_act(x, self.num_groups, self.weight, self.bias, self.eps, self.act, p, self.seed,
-                           self.offset if p > 0 else 0)
-        if p > 0:
+        if p == 0:
+            return group_norm_act(x, self.num_groups, self.weight, self.bias, self.eps, self.act)
+        y = group_norm_act(x, self.num_groups, self.weight, self.bias, self.eps, self.act, p, self.seed, _next_offset(self, offset))
+        if offset is None:
             self.offset.add_(1)
         return y
 
@@ -81,9 +97,10 @@ class CounterDropout(nn.Module):
         self.p, self.seed = p, seed
         self.register_buffer("offset", torch.zeros(1, dtype=torch.int64))
 
-    def forward(self, x, residual=None):
+    def forward(self, x, residual=None, offset=None):
         if not self.training or self.p == 0:
             return x if residual is None else x + residual
-        y = counter_dropout(x, self.p, self.seed, self.offset, residual)
-        self.offset.add_(1)
+        y = counter_dropout(x, self.p, self.seed, _next_offset(self, offset), residual)
+        if offset is None:
+            self.offset.add_(1)
         return y

@@ -324,6 +324,10 @@ class Generator(nn.Module):
     def forward(self, rain_lr, dem, lu, input_grid_size=None):
         """rain_lr [B,T,1,H,W], dem [B,1,Hd,Wd], lu [B,L,Hl,Wl] -> [B,T,1,Hh,Wh] (fp32)."""
         from .autograd import _param_list, rollout_with_grad
+        drops = self.feature_norm is not None and self.feature_norm.training and self.feature_norm.p > 0
+        if drops and ops._inside_backward():
+            raise RuntimeError("a Generator with dropout in its feature head runs inside a backward pass (activation recomputation?), "
+                               "where the mask would be another one than before")
         home = rain_lr.device if isinstance(rain_lr, torch.Tensor) else None
         if isinstance(rain_lr, torch.Tensor) and not rain_lr.is_cuda:
             # CPU-resident caller (the reference's test/test_model.py builds model and inputs on the
@@ -347,7 +351,7 @@ class Generator(nn.Module):
             out = rollout_with_grad(self, rain_lr, dem, lu, input_grid_size, params)
         else:
             out = self._forward_impl(rain_lr, dem, lu, input_grid_size, False, [p.detach() for p in params])[0]
-        if self.feature_norm is not None and self.feature_norm.training and self.feature_norm.p > 0:
+        if drops:
             self.feature_norm.offset.add_(1)          # (on the device: a captured step draws a new mask on every replay)
         return out if out.device == home else out.to(home)
 

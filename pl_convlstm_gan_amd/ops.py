@@ -130,6 +130,11 @@ def _draw(seed, offset):
     return seed, offset, None
 
 
+def _inside_backward() -> bool:
+    """Whether this thread is running a backward pass, as where activations are recomputed."""
+    return torch._C._current_graph_task_id() != -1
+
+
 def gated_scan_forward(x, f, h0=None, lengths=None, coupled=True, save_states=False, h_last=None):
     """plc_gated_scan_fwd on [B, T, ...]: returns (y, h_last, states); states (what the backward pass needs beside the
     inputs) is None unless ``save_states`` and T > 8.  ``h_last``: where the last state goes (may be h0 itself)."""

@@ -53,3 +53,91 @@ def test_recorders_that_cannot_see_a_kernel_are_refused():
                 torch.jit.trace(call, (a, b), check_trace=False)
             with pytest.raises(RuntimeError, match="record"):
                 make_fx(call)(a, b)
+
+
+@pytest.fixture
+def cpu_stand_ins(monkeypatch):
+    """The two operators with a mask, computed by the 64-bit references' generator on the CPU."""
+    import layer_refs as R
+    from pl_convlstm_gan_amd import layers
+
+    def mask(x, p, seed, offset):
+        return (R.keep_mask(x.numel(), p, int(seed), int(offset)).float() * R.keep_scale(p)).view(x.shape) if p > 0 else torch.ones(x.shape)
+
+    def dropout(x, p, seed, offset=0, residual=None):
+        y = x * mask(x, p, seed, offset)
+        return y if residual is None else y + residual
+
+    def norm(x, groups, w=None, b=None, eps=1e-5, act="none", p=0.0, seed=0, offset=0):
+        y = torch.nn.functional.group_norm(x, groups, w, b, eps)
+        return y * mask(y.permute(0, 2, 3, 1), p, seed, offset).permute(0, 3, 1, 2)
+    monkeypatch.setattr(layers, "counter_dropout", dropout)
+    monkeypatch.setattr(layers, "group_norm_act", norm)
+    return layers
+
+
+def recomputed(layers, dev, reentrant):
+    """Activation recomputation runs a module's forward a second time inside the backward pass, when its own offset has moved on:
+    refused, and right with an offset that the caller gives."""
+    from torch.utils.checkpoint import checkpoint
+    x = torch.randn(2, 8, 6, 5, device=dev).contiguous(memory_format=torch.channels_last).requires_grad_()
+    for m in (layers.CounterDropout(0.5, seed=1).to(dev), layers.GroupNormAct(4, 8, p=0.5, seed=1).to(dev)):
+        y = checkpoint(lambda v: m(v).square(), x, use_reentrant=reentrant)
+        with pytest.raises(RuntimeError, match="offset"):
+            y.sum().backward()
+        before = int(m.offset)
+        for offset in (7, torch.tensor([7], device=dev)):
+            plain = torch.autograd.grad(m(x, offset=offset).square().sum(), x)[0]
+            y = checkpoint(lambda v, k: m(v, offset=k).square(), x, offset, use_reentrant=reentrant)
+            x.grad = None
+            y.sum().backward()
+            assert torch.equal(x.grad, plain) and int(m.offset) == before
+        if isinstance(m, layers.CounterDropout):
+            assert torch.equal(y == 0, x.grad == 0) and bool((y == 0).any())
+        # without a mask there is nothing to keep apart
+        m.eval()
+        want = torch.autograd.grad(m(x).square().sum(), x)[0]
+        x.grad = None
+        checkpoint(lambda v: m(v).square(), x, use_reentrant=reentrant).sum().backward()
+        assert torch.equal(x.grad, want)
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_recomputation_takes_the_same_mask_or_raises(cpu_stand_ins, reentrant):
+    recomputed(cpu_stand_ins, torch.device("cpu"), reentrant)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_recomputation_on_the_gpu(gpu, reentrant):
+    from pl_convlstm_gan_amd import layers
+    recomputed(layers, gpu, reentrant)
+
+
+def test_generator_with_a_mask_is_not_recomputed():
+    """The rollout with the feature head's dropout inside a backward pass: refused before anything runs; without dropout, or
+    in evaluation mode, it is not (and a machine without a GPU is the complaint)."""
+    from pl_convlstm_gan_amd import Generator
+
+    class Probe(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, call):
+            ctx.call = call
+            return x * 1
+
+        @staticmethod
+        def backward(ctx, g):
+            ctx.call()
+            return g, None
+    model = Generator(hidden_dims=[16, 32], lu_channels=5, scale_factor=1)
+    args = torch.zeros(1, 2, 1, 16, 16), torch.zeros(1, 1, 16, 16), torch.zeros(1, 5, 16, 16)
+
+    def inside():
+        with pytest.raises(RuntimeError) as e:
+            model(*args) if not torch.cuda.is_available() else pytest.skip("needs a machine without a GPU")
+        messages.append(str(e.value))
+    messages = []
+    for p, training in ((0.0, True), (0.3, False), (0.3, True)):
+        model.set_feature_head(4, p=p, seed=3).train(training)
+        Probe.apply(torch.ones(1, requires_grad=True), inside).backward()
+    assert ["dropout" in m and "backward" in m for m in messages] == [False, False, True]
