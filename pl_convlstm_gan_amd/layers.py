@@ -53,6 +53,14 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, act="none", 
     return _lib.binding().norm(x, num_groups, weight, bias, eps, ops._act(act), p, seed, offset, offset_t)
 
 
+def _first_offset(p, seed):
+    """-> (seed, first offset): without a seed, a point of seed 0's 2^64 offsets drawn from torch's generator, so that modules
+    have masks of their own, torch.manual_seed repeats them and the state_dict holds where they are."""
+    if seed is None and p > 0:
+        return 0, torch.randint(0, 1 << 62, (1,), dtype=torch.int64)
+    return seed or 0, torch.zeros(1, dtype=torch.int64)
+
+
 def _next_offset(module, offset):
     """The offset of a module's pass: the caller's, or the module's own, of which a pass that runs a second time inside the
     backward pass would read another value than the first time."""
@@ -67,17 +75,21 @@ def _next_offset(module, offset):
 class GroupNormAct(nn.Module):
     """group_norm_act with its parameters; ``p``: dropout of the training mode.  The dropout's offset is a buffer that
     every training pass advances by one on the device, so passes draw different masks, replays of a captured pass too.
+    Without a ``seed`` its first value is drawn from torch's default generator, and modules draw masks of their own (copies of
+    one module the same, as they share its offset; a module made with ``p`` = 0 draws nothing).  With one it counts from 0, and
+    modules that share a seed share their masks.
 
     Where a pass is recomputed (torch.utils.checkpoint), give ``forward`` the ``offset`` of the pass, an integer or an int64 tensor
     that nothing changes before the backward pass is done; the buffer is then neither read nor advanced.  Without it a
     recomputation raises: the buffer has moved on by then."""
 
-    def __init__(self, num_groups, num_channels, act="none", p=0.0, eps=1e-5, affine=True, seed=0):
+    def __init__(self, num_groups, num_channels, act="none", p=0.0, eps=1e-5, affine=True, seed=None):
         super().__init__()
-        self.num_groups, self.num_channels, self.act, self.p, self.eps, self.seed = num_groups, num_channels, act, p, eps, seed
+        self.num_groups, self.num_channels, self.act, self.p, self.eps = num_groups, num_channels, act, p, eps
+        self.seed, offset = _first_offset(p, seed)
         self.weight = nn.Parameter(torch.ones(num_channels)) if affine else None
         self.bias = nn.Parameter(torch.zeros(num_channels)) if affine else None
-        self.register_buffer("offset", torch.zeros(1, dtype=torch.int64))
+        self.register_buffer("offset", offset)
 
     def forward(self, x, offset=None):
         p = self.p if self.training else 0.0
@@ -90,12 +102,13 @@ class GroupNormAct(nn.Module):
 
 
 class CounterDropout(nn.Module):
-    """counter_dropout in training mode, the identity (plus ``residual``) otherwise; the offset as in GroupNormAct."""
+    """counter_dropout in training mode, the identity (plus ``residual``) otherwise; the seed and the offset as in GroupNormAct."""
 
-    def __init__(self, p, seed=0):
+    def __init__(self, p, seed=None):
         super().__init__()
-        self.p, self.seed = p, seed
-        self.register_buffer("offset", torch.zeros(1, dtype=torch.int64))
+        self.p = p
+        self.seed, offset = _first_offset(p, seed)
+        self.register_buffer("offset", offset)
 
     def forward(self, x, residual=None, offset=None):
         if not self.training or self.p == 0:

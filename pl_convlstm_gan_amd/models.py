@@ -143,11 +143,11 @@ class Generator(nn.Module):
         if "feature_norm" not in self.__dict__ and "feature_norm" not in self._modules:      # (pickled before the head existed)
             self.feature_norm = None
 
-    def set_feature_head(self, num_groups, act="silu", p=0.0, seed=0):
+    def set_feature_head(self, num_groups, act="silu", p=0.0, seed=None):
         """Adds group norm + activation (+ dropout of probability ``p`` in training mode) on the recurrence's features, in front
         of the upsample blocks.  Not a constructor argument: the reference has none, and without this call the model, its
         parameters and its state_dict are the reference's.  To be called before an optimizer takes the parameters; the head's own
-        are ``feature_norm.weight`` and ``feature_norm.bias``.  ``num_groups`` = 0 removes it."""
+        are ``feature_norm.weight`` and ``feature_norm.bias``.  ``seed`` as in GroupNormAct.  ``num_groups`` = 0 removes it."""
         if num_groups == 0:
             self.feature_norm = None
             return self
@@ -159,7 +159,7 @@ class Generator(nn.Module):
         ops._act(act)
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"p must be a probability (got {p})")
-        ops._draw(seed, 0)
+        ops._draw(0 if seed is None else seed, 0)
         from .layers import GroupNormAct
         self.feature_norm = GroupNormAct(num_groups, ch, act, p, seed=seed).to(self.init_conv.weight.device)
         return self

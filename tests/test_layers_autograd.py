@@ -141,3 +141,62 @@ def test_generator_with_a_mask_is_not_recomputed():
         model.set_feature_head(4, p=p, seed=3).train(training)
         Probe.apply(torch.ones(1, requires_grad=True), inside).backward()
     assert ["dropout" in m and "backward" in m for m in messages] == [False, False, True]
+
+
+def test_default_modules_draw_masks_of_their_own(cpu_stand_ins):
+    """Two modules that were given no seed drop different elements, from the first pass on; torch.manual_seed and a saved
+    state bring the masks back; with a seed the offset counts from 0."""
+    layers = cpu_stand_ins
+    x = torch.ones(2, 8, 16, 16)
+    image = torch.randn(x.shape, generator=torch.Generator().manual_seed(1))
+
+    def make():
+        return torch.nn.ModuleList([layers.CounterDropout(0.5), layers.CounterDropout(0.5), layers.GroupNormAct(2, 8, p=0.5), layers.GroupNormAct(2, 8, p=0.5)])
+
+    def masks(ms):                                         # (of three passes; elements in the order the masks count them)
+        return [torch.stack([ms[0](x) != 0, ms[1](x) != 0] + [(m(image) != 0).permute(0, 2, 3, 1).reshape(x.shape) for m in ms[2:]]) for _ in range(3)]
+    torch.manual_seed(11)
+    a, b = make(), make()
+    got = torch.cat(masks(a) + masks(b)).flatten(1)
+    # 4096 independent fair elements each: the number two masks agree on is 2048 +- 32, 8 deviations allowed
+    agree = (got[:, None] == got[None]).sum(2)
+    agree.fill_diagonal_(2048)
+    assert int((agree - 2048).abs().max()) <= 256
+    torch.manual_seed(11)
+    again = make()
+    assert torch.equal(torch.cat(masks(again)).flatten(1), got[:12])
+    state = {k: v.clone() for k, v in again.state_dict().items()}
+    went_on = torch.cat(masks(again))
+    torch.manual_seed(12)
+    other = make()
+    assert not torch.equal(torch.cat(masks(other)).flatten(1), got[:12])
+    other.load_state_dict(state)
+    assert torch.equal(torch.cat(masks(other)), went_on)
+    for m in (layers.CounterDropout(0.5, seed=0), layers.CounterDropout(0.5, seed=7), layers.GroupNormAct(2, 8, p=0.5, seed=0), layers.CounterDropout(0.0), layers.GroupNormAct(2, 8)):
+        assert int(m.offset) == 0
+    # (nothing is drawn where nothing is dropped, or where a seed is given)
+    torch.manual_seed(3)
+    layers.CounterDropout(0.0), layers.GroupNormAct(2, 8), layers.CounterDropout(0.5, seed=1)
+    drawn = torch.rand(1)
+    torch.manual_seed(3)
+    assert torch.equal(torch.rand(1), drawn)
+
+
+def test_default_feature_heads_draw_masks_of_their_own():
+    from pl_convlstm_gan_amd import Generator
+    make = lambda **kw: Generator(hidden_dims=[16, 32], lu_channels=5, scale_factor=1).set_feature_head(4, p=0.2, **kw).feature_norm  # noqa: E731
+    torch.manual_seed(5)
+    a, b = make(), make()
+    torch.manual_seed(5)
+    assert int(a.offset) != int(b.offset) and int(make().offset) == int(a.offset) and a.seed == b.seed == 0
+    assert int(make(seed=3).offset) == 0 and make(seed=3).seed == 3
+
+
+@pytest.mark.gpu
+def test_default_modules_on_the_gpu(gpu):
+    from pl_convlstm_gan_amd import layers
+    a, b = layers.CounterDropout(0.5).to(gpu), layers.CounterDropout(0.5).to(gpu)
+    x = torch.ones(4096, device=gpu)
+    first, start = int(a.offset), a(x)
+    assert not torch.equal(start, b(x)) and int(a.offset) == first + 1
+    assert torch.equal(start, layers.counter_dropout(x, 0.5, 0, first))
