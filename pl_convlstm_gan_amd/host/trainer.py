@@ -163,8 +163,8 @@ class Trainer:
             torch.manual_seed(0)      # identical initial weights on every rank
         self.model = self._make_model(**kw).to(self.device)
         if getattr(mc, "feature_groups", 0):
-            # (a mask of its own on every rank)
-            self.model.set_feature_head(mc.feature_groups, mc.feature_act, mc.feature_dropout, seed=rank)
+            # (the first offset is drawn, as the weights are; the seed gives every rank a mask of its own)
+            self.model.set_feature_head(mc.feature_groups, mc.feature_act, mc.feature_dropout).feature_norm.seed = rank
         tr = self.config.training
         self.optimizer = self._make_optimizer(self.model.parameters(), tr.learning_rate)
         self.scheduler = torch.optim.lr_scheduler.ReduceLROnPlateau(self.optimizer, mode="min", factor=tr.scheduler_factor,

@@ -200,3 +200,30 @@ def test_default_modules_on_the_gpu(gpu):
     first, start = int(a.offset), a(x)
     assert not torch.equal(start, b(x)) and int(a.offset) == first + 1
     assert torch.equal(start, layers.counter_dropout(x, 0.5, 0, first))
+
+
+def test_trainer_runs_and_ranks_draw_masks_of_their_own(monkeypatch):
+    """Two runs of the Trainer draw different masks unless torch's seed is the same; ranks start at one offset (and one set of
+    weights) under seeds of their own."""
+    from pl_convlstm_gan_amd.host import trainer as T
+    from pl_convlstm_gan_amd.host.config import Config
+
+    class Data:
+        lucc_onehot = torch.zeros(5, 4, 4)
+
+    def head(rank=0, world=1, dropout=0.2):
+        monkeypatch.setattr(T, "_rank_world", lambda: (rank, world))
+        t = T.Trainer.__new__(T.Trainer)
+        t.config, t.device = Config(), torch.device("cpu")
+        t.config.model.feature_groups, t.config.model.feature_dropout = 4, dropout
+        t._make_optimizer = lambda params, lr: torch.optim.Adam(params, lr=lr)
+        t.setup_model(Data())
+        return t.model.feature_norm.seed, int(t.model.feature_norm.offset), t.model.init_conv.weight.detach().clone()
+    torch.manual_seed(1)
+    (s0, o0, _), (s1, o1, _) = head(), head()
+    assert o0 != o1 and s0 == s1 == 0
+    torch.manual_seed(1)
+    assert head()[1] == o0
+    (s0, o0, w0), (s1, o1, w1) = head(0, 2), head(1, 2)
+    assert (s0, s1) == (0, 1) and o0 == o1 and torch.equal(w0, w1)
+    assert head(dropout=0.0)[:2] == (0, 0)
