@@ -59,6 +59,48 @@ def scan(x, f, h0, lengths, coupled, dy=None, dh=None):
     return {k: v.to(dev) for k, v in val.items()}, {k: v.to(dev) for k, v in err.items()}
 
 
+def _linear(a, b):
+    """h[:, t] = a[:, t] h[:, t - 1] + b[:, t], h before the first step 0, by doubling the reach of each step."""
+    d = 1
+    while d < a.shape[1]:
+        b = torch.cat([b[:, :d], b[:, d:] + a[:, d:] * b[:, :-d]], 1)
+        a = torch.cat([a[:, :d], a[:, d:] * a[:, :-d]], 1)
+        d *= 2
+    return b
+
+
+def scan_long(x, f, h0, lengths, coupled, dy, dh):
+    """scan() for sequences of which a loop over the steps takes too long: values and bounds are linear recurrences all."""
+    dev = x.device
+    x, f, h0, dy, dh = (t.detach().cpu().double() for t in (x, f, h0, dy, dh))
+    B, T = x.shape[:2]
+    n = torch.full((B,), T) if lengths is None else lengths.cpu().clamp(0, T).long()
+    on = (torch.arange(T)[None] < n[:, None]).view((B, T) + (1,) * (x.dim() - 2))
+    zero = torch.zeros((), dtype=torch.float64)
+    s, q = torch.sigmoid(f), torch.sigmoid(-f)
+    a = torch.where(on, s, 1.0)
+    start = lambda b, v: torch.cat([b[:, :1] + a[:, :1] * v[:, None], b[:, 1:]], 1)  # noqa: E731
+    h = _linear(a, start(torch.where(on, q * x if coupled else x, zero), h0))
+    before = torch.cat([h0[:, None], h[:, :-1]], 1)
+    E = _linear(a, torch.where(on, 16 * U * (before.abs() + x.abs()), zero))
+    Eb = torch.cat([torch.zeros_like(E[:, :1]), E[:, :-1]], 1)
+    back = lambda b: _linear(a.flip(1), b.flip(1)).flip(1)  # noqa: E731
+    behind = lambda c, last: torch.cat([c[:, 1:], last[:, None]], 1)  # noqa: E731
+    inner = torch.where(on, a * dy, zero)
+    g = back(torch.cat([inner[:, :-1], inner[:, -1:] + a[:, -1:] * dh[:, None]], 1))          # what a step passes to the one in front of it
+    full = behind(g, dh) + dy
+    step = 2 * U * (behind(g, dh).abs() + dy.abs())
+    Eg = back(torch.where(on, a * (step + 16 * U * full.abs()), zero))
+    Efull = behind(Eg, torch.zeros_like(dh)) + step
+    m = before - x if coupled else before
+    Em = Eb + 2 * U * (before.abs() + (x.abs() if coupled else 0))
+    k = q if coupled else torch.ones_like(q)
+    val = {"y": torch.where(on, h, zero), "h_last": h[:, -1], "dx": torch.where(on, full * k, zero), "df": torch.where(on, full * m * s * q, zero), "dh0": g[:, 0]}
+    err = {"y": torch.where(on, E, zero), "h_last": E[:, -1], "dx": torch.where(on, k * (Efull + 16 * U * full.abs()), zero),
+           "df": torch.where(on, s * q * (Efull * m.abs() + full.abs() * (Em + 32 * U * m.abs())), zero), "dh0": Eg[:, 0]}
+    return {k: v.to(dev) for k, v in val.items()}, {k: v.to(dev) for k, v in err.items()}
+
+
 def philox(ctr, key):
     """Philox4x32-10 on arrays of 32-bit words held in uint64: ctr four arrays, key two integers -> four arrays."""
     low, s32 = np.uint64(0xFFFFFFFF), np.uint64(32)
