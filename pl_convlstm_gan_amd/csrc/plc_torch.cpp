@@ -122,6 +122,7 @@ torch::autograd::variable_list once(torch::autograd::variable_list grads, const 
 // backward pass) down to the leaves.  A graph made on the default stream before the capture may stay outside that pass, so it is
 // looked at when a backward pass of these operators is about to lead there.
 bool capturing(const c10::hip::HIPStream& stream) {
+    if (!stream.stream()) return false;      // (the default stream; asking the runtime takes a microsecond of a training call)
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     return hipStreamIsCapturing(stream.stream(), &status) == hipSuccess && status != hipStreamCaptureStatusNone;
 }
