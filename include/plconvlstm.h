@@ -422,6 +422,7 @@ enum { PLC_F32 = 0, PLC_BF16 = 1, PLC_F16 = 2 };
  * one); y, dx, df are contiguous [B][T][D]; h0, h_last, dh_last, dh0 are fp32 [B][D].
  *   lengths  NULL or int32 [B] on the device: sample b has min(max(lengths[b], 0), T) steps.  Behind them y, dx and df
  *            are 0, whatever x, f and dy hold there, and the state stands still (h_last of a sample without a step is h0).
+ *   x        an infinite one, or coupled an x - h beyond fp32's range, makes the states behind it infinite or NaN
  *   h0       NULL = zeros;  h_last NULL = not wanted, else it may be h0 itself (a state updated in place)
  *   states   forward: NULL, or room for plc_gated_scan_states_bytes(B, T, D) bytes that the backward pass reads
  *            (the fp32 state in front of every 8th step; none for T <= 8, where NULL serves the backward pass too)

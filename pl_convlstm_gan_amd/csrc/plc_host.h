@@ -1,5 +1,5 @@
 // Host-side helpers shared by the library's translation units: the error message of the calling thread, argument
-// checks, small integer arithmetic, the CU count of the current device.
+// checks, small integer arithmetic.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -10,7 +10,6 @@
 
 // stores the message plc_last_error() returns on this thread and gives `code` back
 PLC_HIDDEN int plc_fail(int code, const char* fmt, ...);
-// number of CUs of the current device (looked up once per device)
 
 #define PLC_HIP(expr)                                                                         \
     do {                                                                                      \

@@ -32,6 +32,9 @@ struct VecRule {
 // In us, kept against streamed, in brackets with a reader of the output behind it:
 //   scan forward, bf16   84 MB 49.5 (81.8) 53.9 (79.3)   126 MB 83.5 (129) 79.4 (119)   168 MB 110 (167) 97 (150)   335 MB 218 (320) 230 (343)
 //   dropout + residual   84 MB 42.9 (70.8) 44.2 (70.0)   126 MB 69.2 (112) 62.0 (102)   168 MB 91.6 (151) 87.3 (138)   335 MB 177 (286) 168 (291)
+//   dropout              84 MB 31.1 (56.5) 28.9 (53.2)   126 MB 44.4 (85.5) 41.6 (80.0)   168 MB 58.8 (115) 57.7 (111)   250 MB 84.3 (167) 85.1 (170)   335 MB 112 (219) 112 (226)
+// (Dropout alone has one input; the one range serves both.  fp32 dropout does not stream at any size: a lane moves 32 bytes of it
+// in two accesses, and the form was not built for it.)
 // (Not where a backward pass will read the scan's inputs again: a training pass of 168 MB tensors takes 316 us with it, 309 without.)
 static bool streams(double bytes) { return bytes > 100e6 && bytes < 256e6; }
 

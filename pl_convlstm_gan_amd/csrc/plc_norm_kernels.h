@@ -20,8 +20,13 @@
 // was slower, 157 us, as was going through the tensor in chunks of samples that fit the caches (113 to 182).
 // 80 samples of 128 x 128 x 32 with silu and dropout: 20.1 + 43.4 us forward, 56.0 + 54.1 backward; there the generator (ten
 // rounds per eight elements) and the exponential cost as much as the memory.
-// Resident: 5 x 15 x 12 x 32 fp32 3.9 us forward, one launch of 20 workgroups, all latency; 8 x 32 x 32 x 512 fp16 9 us
-// forward (17 MB: 1.9 TB/s) and 15 + 4 backward, the last for dw and db.
+// Resident: 5 x 15 x 12 x 32 fp32 4.2 us forward, one launch of 40 workgroups of a wave, all latency; 8 x 32 x 32 x 512 fp16 9.5 us
+// forward (17 MB: 1.8 TB/s) and 15 + 4 backward, the last a launch of its own for dw and db, which are sums over samples that
+// different workgroups hold.
+// Narrow units (a C without a common factor with the vector) cost the generator, which is called per unit: 40 x 256 x 256 bf16 with
+// dropout, forward/backward, 32 channels 96/163 us, 30 (units of two) 165/279, 31 (of one) 294/515; without it 87/147, 87/179, 105/200.
+// Many groups cost the split form's joining of the partial sums, which every workgroup does for all groups of its tile:
+// 4 x 128 x 128 x 512 bf16 61/77 us with 32 groups, 405/265 with 512.
 #pragma once
 #include "plc_layers_common.h"
 
@@ -137,8 +142,8 @@ __device__ __forceinline__ float norm_block_sum(float v, float* scratch) {
 }
 
 // Sums over the rows where the lanes of a wave that hold one unit are those that agree modulo nu (NHWC rows of 1, 2, 4, 8 or 16 units;
-// CB8 tiles of one): added across the lanes, then one value per wave.  Two barriers and no more LDS than the result times the
-// number of waves; the general form below has four and moves every value through LDS.
+// CB8 tiles of one): added across the lanes, then one value per wave.  Three barriers and no more LDS than the result times the
+// number of waves; the general form below has five (three where a channel is one thread's) and moves every value through LDS.
 template <int V, int NV, int NU>
 __device__ __forceinline__ void norm_sum_waves(const float (&v)[NV][V], float* scratch, float* out) {
     constexpr int nch = NU * V;
@@ -453,8 +458,10 @@ __device__ __forceinline__ float norm_entry_count(const NormArgs& a, int V, int 
 
 // ---- split form, forward, second pass ---------------------------------------------------------------------------
 // Nothing it touches is needed in the caches afterwards, and what the first pass left of x there is: loads and stores stream.
-// bf16, 32 channels in 8 groups, both passes together: 40 x 256 x 256 86.4 us against 104.4, 20 x 128 x 128 19.5 against 20.6; with
-// an operator that reads y behind them 160 against 172 and 30.5 against 30.9.  (Streaming in the first pass too: 93.8.)
+// 32 channels in 8 groups, both passes together, in brackets with an operator that reads y behind them, against loads and stores that
+// stay: bf16 40 x 256 x 256 84.4 (152) us against 104 (162), 12 x 256 x 256 30.0 (47.1) against 31.5 (48.1), 20 x 128 x 128 18.7 (28.1)
+// against 20.5 (28.5), 2 x 256 x 256 15.1 (21.2) against 16.0 (21.5), 4 x 128 x 128 14.5 (18.7) both; fp32 2 x 256 x 256 15.4 (22.8)
+// against 16.6 (22.7).  (Streaming in the first pass too, 40 x 256 x 256: 93.8 where this took 86.4.)
 template <class T, int V, int FORM>
 __global__ __launch_bounds__(256) void plc_norm_fwd_kernel(NormArgs a) {
     extern __shared__ __align__(16) float st[];

@@ -45,7 +45,8 @@ __device__ __forceinline__ bool scan_open(float w) { return __builtin_bit_cast(i
 __device__ __forceinline__ float scan_s(float w) { return scan_open(w) ? 1.0f + w : w; }
 
 // One step.  The coupled form is a mean of h and x: it starts from the one with the larger weight and moves by the smaller
-// weight times the difference, which is exact at h = x and at s = 0 and 1, and loses nothing of a gate near 1.
+// weight times the difference, which is exact at h = x and at s = 0 and 1, and loses nothing of a gate near 1.  (The price: an
+// infinite x, or an x - h beyond fp32's range, gives an infinity or a NaN where the two products would give their sum.)
 template <bool COUPLED>
 __device__ __forceinline__ float scan_step(float h, float x, float w) {
     if (!COUPLED) return __builtin_fmaf(scan_s(w), h, x);
@@ -228,8 +229,8 @@ __global__ __launch_bounds__(256) void plc_scan_bwd_kernel(ScanArgs a) {
 // front of (the gradient behind) each, the third walks the segments as above.  x and f (f and dy) are read twice, the second
 // time mostly from the cache; in return every segment runs at once.  Lanes run over (segment, channels): a row of few
 // channels does not leave lanes of a wave idle.
-// 4 x 32768 x 96 bf16 with lengths: 12.0 + 6.2 + 18.4 us (75 MB that cannot be done without, 126 MB moved); 8 x 3653 x 48 fp32
-// forward 5.1 + 6.0 + 5.6 us, backward 4.4 + 5.8 + 5.9: three launches of which none is bound by memory.
+// 4 x 32768 x 96 bf16 with lengths: 12.8 + 5.8 + 18.7 us (75 MB that cannot be done without, 126 MB moved); 8 x 3653 x 48 fp32
+// forward 5.3 + 6.2 + 5.5 us, backward 4.6 + 5.9 + 6.1: three launches of which none is bound by memory.
 template <int V>
 __device__ __forceinline__ bool scan_item(const ScanArgs& a, ScanLane& l, int& k) {
     const unsigned lanes = (unsigned)(a.B * (a.D / V)), i = blockIdx.x * blockDim.x + threadIdx.x;

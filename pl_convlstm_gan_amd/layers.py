@@ -21,7 +21,8 @@ def gated_linear_scan(x, f, h0=None, lengths=None, coupled=True):
 
     ``h0``: float32 [B, ...], the state in front of the first step (default zeros).  ``lengths``: int32 [B] on x's
     device; behind a sample's length the outputs and gradients are 0, whatever the padding holds, and its state stands
-    still.  An infinite x makes the states behind it infinite or NaN.  Strided x and f are read in place as long as their trailing dimensions are contiguous."""
+    still.  An infinite x makes the states behind it infinite or NaN, and so does, coupled, an x - h beyond float32's range.
+    Strided x and f are read in place as long as their trailing dimensions are contiguous."""
     return _lib.binding().scan(x, f, h0, lengths, coupled)
 
 
